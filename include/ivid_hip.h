@@ -279,6 +279,37 @@ int ivid_gn_apply_p(int dtype, const void* src0, const void* src0_lo, int C0, co
                     const float* ab, void* out, void* pool_hi, void* pool_lo, int N, int H, int W, int resample, int act,
                     void* stream);
 
+/* ---- GroupNorm + FiLM + activation + dropout with its gradient: the trainable form of the norms above ----
+ * (`out_layers[:3]` of a ResBlock: GroupNorm32, FiLM, SiLU, Dropout, adm.py:177-189,214-218; `in_layers[:2]` on the skip concat,
+ * adm.py:157-160,563; the attention block's norm, adm.py:274,281.)
+ *   y = drop(act(u * (1 + scale) + shift)),  u = xhat * gamma + beta,  xhat = (x - mean) * rstd
+ * x = cat[src0, src1] over channels, N samples of HW pixels; mean and biased variance per (sample, group) in fp32 or wider;
+ * act 0 none, 1 SiLU; drop as in ivid_dropout, element index = row-major index in the [N,HW,C0+C1] output.
+ * Any HW >= 1, any C0 + C1 divisible by groups, any element alignment. */
+typedef struct {
+  int dtype;                              /* IVID_F32, IVID_BF16 or IVID_F16: src, out, dy, dsrc */
+  int N, HW, C0, C1, groups, act;         /* C1 = 0 and src1 = NULL: one source */
+  const void* src0; long long ld0, sn0;   /* channels contiguous; elements from a pixel / a sample to the next */
+  const void* src1; long long ld1, sn1;
+  const float* gamma; const float* beta;  /* [C0+C1] */
+  const void* film;                       /* NULL, or rows of 2*(C0+C1): scale then shift, film_ld elements from a row to the next */
+  int film_dtype; long long film_ld;      /* IVID_F32 or `dtype` */
+  double eps, p;                          /* p = 0: no dropout */
+  unsigned long long seed, stream_id;     /* of the dropout draws */
+  const unsigned long long* rng;          /* NULL, or device {seed, stream_id}: replaces the two above, read when the kernel runs */
+} ivid_gn_act_desc;
+/* Device scratch of one call in bytes (8-byte aligned), -1 for a malformed descriptor.  Contents need not be kept between calls,
+ * nor between a forward and its backward; two calls that may run at once need a scratch each. */
+long long ivid_gn_act_scratch_bytes(const ivid_gn_act_desc* host_desc, int backward);
+/* out [N,HW,C0+C1]; stats fp32 [N,groups,2] = mean, rstd (what the backward pass needs) */
+int ivid_gn_act_forward(const ivid_gn_act_desc* host_desc, void* out, float* stats, void* scratch, long long scratch_bytes,
+                        void* stream);
+/* dy [N,HW,C0+C1] contiguous -> dsrc0 [N,HW,C0], dsrc1 [N,HW,C1] (NULL iff C1 = 0), dgamma, dbeta fp32 [C0+C1], dfilm [N, 2*(C0+C1)]
+ * contiguous in film_dtype (NULL iff no film).  The descriptor and stats of the forward call; xhat, the activation and the
+ * dropout draws are computed again, no mask or activation is kept.  Deterministic: no atomics. */
+int ivid_gn_act_backward(const ivid_gn_act_desc* host_desc, const float* stats, const void* dy, void* dsrc0, void* dsrc1,
+                         float* dgamma, float* dbeta, void* dfilm, void* scratch, long long scratch_bytes, void* stream);
+
 /* ---- QKVAttention (adm.py:233-253), legacy per-head [q|k|v] channel interleave ----
  * qkv: NHWC [N,T,3*C] with channel = head*192 + {0..63 q, 64..127 k, 128..191 v}; out: [N,T,C], channel = head*64+d.
  * softmax in fp32 (adm.py:251); scores scaled by 64^-1/2 overall (q*64^-1/4 . k*64^-1/4, adm.py:247-250). */
@@ -365,6 +396,16 @@ int ivid_sr_cond(const float* x, const float* y, float* out, int B, int Cx, int 
  * values, 24-bit uniforms, Box-Muller -- so that a chain's noise needs no buffers and does not depend on launch shapes, ranks
  * or call order.  out: device fp32, 16-byte aligned. */
 int ivid_randn(unsigned long long seed, unsigned long long stream_id, float* out, long long n, void* stream);
+
+/* ---- dropout (nn.Dropout of a ResBlock, adm.py:181) from the same generator, the mask never stored ----
+ * out[i] = kept(i) ? x[i] * 65536 / (65536 - T) : 0,  T = floor(p * 65536 + 1/2), kept(i) = draw(i) >= T: the expectation is x for
+ * every p < 1 (p is used in steps of 2^-16); p = 1 drops all.  draw(i) = 16 bits, half i % 2 (low first) of word (i % 8) / 2 of the
+ * Philox4x32-10 block with counter (i / 8, stream_id) and key seed ^ 0x44524F50 << 32: a pure function of (seed, stream_id, i), so the
+ * backward pass is the same call on the gradient, and independent of ivid_randn's values for the same (seed, stream_id).
+ * A dropped element is 0 whatever x holds.  x == out is allowed.  rng: NULL, or device {seed, stream_id} read when the kernel runs
+ * instead of the arguments (a captured graph then draws anew when the host rewrites them between replays). */
+int ivid_dropout(int dtype, const void* x, void* out, long long n, double p, unsigned long long seed, unsigned long long stream_id,
+                 const unsigned long long* rng, void* stream);
 
 /* ---- the whole sampling loop as ONE call (SURVEY.md 8(b) `ivid_sample(handle, plan*, ...)`) ----
  * DdimSampler.sample / DdpmSampler.sample (diffusion/samplers/ddim.py:150-163, ddpm.py:172-185) with the frameworks'

@@ -85,6 +85,15 @@ class SampleCond(C.Structure):      # ivid_sample_cond
                                             "sr_y")] + [("sr_channels", C.c_int), ("sr_size", C.c_int)])
 
 
+class GnActDesc(C.Structure):       # ivid_gn_act_desc
+    _fields_ = ([(n, C.c_int) for n in ("dtype", "N", "HW", "C0", "C1", "groups", "act")]
+                + [("src0", C.c_void_p), ("ld0", C.c_longlong), ("sn0", C.c_longlong),
+                   ("src1", C.c_void_p), ("ld1", C.c_longlong), ("sn1", C.c_longlong),
+                   ("gamma", C.c_void_p), ("beta", C.c_void_p), ("film", C.c_void_p), ("film_dtype", C.c_int),
+                   ("film_ld", C.c_longlong), ("eps", C.c_double), ("p", C.c_double), ("seed", C.c_ulonglong),
+                   ("stream_id", C.c_ulonglong), ("rng", C.c_void_p)])
+
+
 SAMPLE_DDIM, SAMPLE_DDPM = 0, 1
 
 # name -> (restype, argtypes); must list every symbol declared in include/ivid_hip.h
@@ -135,6 +144,9 @@ SIGNATURES = {
     "ivid_gn_finalize": (i32, [vp, i32, i32, i32, i32, i32, C.c_float, vp, vp, vp, i32, i32, vp, vp]),
     "ivid_gn_finalize2": (i32, [vp, i32, i32, vp, i32, i32, i32, i32, i32, C.c_float, vp, vp, vp, i32, i32, vp, vp]),
     "ivid_gn_apply": (i32, [i32, vp, i32, vp, i32, vp, vp, i32, i32, i32, i32, i32, vp]),
+    "ivid_gn_act_scratch_bytes": (i64, [C.POINTER(GnActDesc), i32]),
+    "ivid_gn_act_forward": (i32, [C.POINTER(GnActDesc), vp, vp, vp, i64, vp]),
+    "ivid_gn_act_backward": (i32, [C.POINTER(GnActDesc), vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]),
     "ivid_attention": (i32, [i32, vp, vp, i32, i32, i32, vp]),
     "ivid_embed_inputs": (i32, [vp, vp, i32, i32, i32, vp, i32, vp, i32, vp, vp, vp]),
     "ivid_silu_f32": (i32, [vp, vp, i64, vp]),
@@ -142,6 +154,7 @@ SIGNATURES = {
     "ivid_nchw_to_nhwc": (i32, [i32, vp, i32, i32, i32, i32, i32, i32, vp, vp]),
     "ivid_stem_im2col": (i32, [i32, vp, i32, i32, i32, i32, i32, i32, vp, vp]),
     "ivid_randn": (i32, [C.c_ulonglong, C.c_ulonglong, vp, i64, vp]),
+    "ivid_dropout": (i32, [i32, vp, vp, i64, C.c_double, C.c_ulonglong, C.c_ulonglong, vp, vp]),
     "ivid_sample_scratch_bytes": (i64, [vp, i32, C.POINTER(SamplePlan), C.POINTER(SampleCond)]),
     "ivid_sample": (i32, [vp, i32, C.POINTER(SamplePlan), vp, C.POINTER(SampleCond), vp, vp, vp, vp, i64, vp]),
     "ivid_ddim_step": (i32, [vp, vp, vp, C.POINTER(DdimCoef), vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, vp]),

@@ -9,6 +9,7 @@
 //   - InpaintCFG.make_cond_inputs                                   (inpaint_cfg.py:24-49)
 #include "common.h"
 #include "internal.h"
+#include "philox.h"
 
 namespace {
 
@@ -260,16 +261,6 @@ extern "C" int ivid_copy(void* dst, const void* src, long long bytes, void* stre
 // seed_hi)); a 32-bit word r becomes the uniform u = ((r >> 8) + 0.5) * 2^-24 in (0, 1) -- exact in fp32 --, pairs (u0, u1) become
 // sqrt(-2 ln u0) * (cos, sin)(2 pi u1).  A value depends on (seed, sid, index) alone: any launch shape, any rank, any order.
 namespace {
-__device__ inline void philox4x32_10(uint32_t c[4], uint32_t k0, uint32_t k1) {
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint32_t hi0 = __umulhi(0xD2511F53u, c[0]), lo0 = 0xD2511F53u * c[0];
-    const uint32_t hi1 = __umulhi(0xCD9E8D57u, c[2]), lo1 = 0xCD9E8D57u * c[2];
-    const uint32_t n0 = hi1 ^ c[1] ^ k0, n2 = hi0 ^ c[3] ^ k1;
-    c[0] = n0; c[1] = lo1; c[2] = n2; c[3] = lo0;
-    k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
-  }
-}
 __global__ __launch_bounds__(256) void randn_kernel(unsigned long long seed, unsigned long long sid, float* __restrict__ out, long long n) {
   const long long j = (long long)blockIdx.x * 256 + threadIdx.x;
   if (4 * j >= n) return;

@@ -1,0 +1,443 @@
+"""GPU tests of ivid_amd.functional against the 64-bit references and bounds of functional_ref.py."""
+import numpy as np
+import pytest
+import torch
+
+import common  # noqa: F401
+import functional_ref as R
+
+pytestmark = pytest.mark.gpu
+DTS = [torch.float32, torch.bfloat16, torch.float16]
+RNG = (0x123456789ABCDEF1, 7)
+
+
+def F():
+    from ivid_amd import functional
+    return functional
+
+
+def randn(seed, *shape, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(*shape, generator=g).to("cuda", dtype)
+
+
+def gn_inputs(seed, shape, c0, c1, dtype, film, offset=0.5):
+    """x [*shape, c0], skip, weight, bias, film; shape[0] = N."""
+    c = c0 + c1
+
+    def act(s, ch):
+        x = randn(s, *shape, ch) * (0.5 + torch.rand(ch, generator=torch.Generator().manual_seed(s + 1)).cuda()) + offset * randn(s + 2, ch)
+        return x.to(dtype)
+    return dict(x=act(seed, c0), skip=act(seed + 10, c1) if c1 else None, weight=1 + 0.2 * randn(seed + 20, c),
+                bias=0.2 * randn(seed + 21, c),
+                film=None if film is None else (0.3 * randn(seed + 22, shape[0], 2 * c)).to(dtype if film == "same" else torch.float32))
+
+
+def run_gn(t, groups, dy, **kw):
+    """(outputs as functional_ref names them) through autograd."""
+    names = [k for k in ("x", "skip", "weight", "bias", "film") if t[k] is not None]
+    leaves = {k: t[k].detach().requires_grad_() for k in names}
+    y = F().group_norm_act(leaves["x"], groups, leaves["weight"], leaves["bias"], film=leaves.get("film"), skip=leaves.get("skip"), **kw)
+    out = dict(y=y)
+    out.update(zip(["d" + k for k in names], torch.autograd.grad(y, list(leaves.values()), dy)))
+    with torch.no_grad():
+        y2, out["stats"] = F().group_norm_act_forward(t["x"], groups, t["weight"], t["bias"], film=t["film"], skip=t["skip"], **kw)
+    assert torch.equal(torch.nan_to_num(y2), torch.nan_to_num(y.detach()))
+    return out
+
+
+GN_CASES = [
+    # name, [N, spatial...], C0, C1, groups, film, act, p
+    ("one_value_a_group", (3, 1), 8, 0, 8, "f32", "silu", 0.0),
+    ("two_values_a_group", (2, 1), 64, 0, 32, None, "silu", 0.0),
+    ("one_pixel", (5, 1), 96, 0, 4, "same", "silu", 0.1),
+    ("one_channel", (2, 9, 7), 1, 0, 1, "f32", "none", 0.3),
+    ("bottleneck", (1, 8, 8), 1024, 0, 32, "f32", "silu", 0.0),
+    ("plain_16x16", (3, 16, 16), 256, 0, 32, "same", "silu", 0.1),
+    ("concat_seam_in_a_group", (2, 16, 16), 128, 96, 32, None, "silu", 0.0),
+    ("concat_odd", (2, 5, 3), 33, 18, 17, "f32", "silu", 0.2),
+    ("odd_37x23_c100_g20", (2, 37, 23), 100, 0, 20, "f32", "silu", 0.25),
+    ("odd_c33_g3", (2, 13, 11), 33, 0, 3, "same", "silu", 0.1),
+    ("c36_g6_seq77", (4, 77), 36, 0, 6, None, "none", 0.0),
+    ("one_group_c513", (2, 6, 5), 513, 0, 1, "f32", "silu", 0.1),
+    ("one_group_c1000", (1, 40, 12), 1000, 0, 1, None, "silu", 0.0),
+    ("one_group_wide", (2, 3, 3), 5000, 0, 1, "f32", "silu", 0.5),
+    ("one_channel_a_group", (2, 12, 12), 64, 0, 64, None, "silu", 0.0),
+    ("one_channel_a_group_c200", (2, 9, 30), 200, 0, 200, "f32", "silu", 0.1),
+    ("level0_64x64", (2, 64, 64), 64, 0, 32, "f32", "silu", 0.1),
+    ("seq1024_c512", (2, 1024), 512, 0, 32, None, "none", 0.0),
+    ("tall_128x128", (1, 128, 128), 128, 0, 32, "f32", "silu", 0.0),
+    ("ragged_131x127_c48", (1, 131, 127), 48, 0, 8, None, "silu", 0.1),
+    ("p_one", (2, 4, 4), 32, 0, 8, "f32", "silu", 1.0),
+    ("many_samples", (300, 2, 2), 32, 0, 8, "f32", "silu", 0.1),
+]
+
+
+@pytest.mark.parametrize("dtype", DTS, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("case", GN_CASES, ids=[c[0] for c in GN_CASES])
+def test_group_norm_act_and_its_gradients(case, dtype):
+    name, shape, c0, c1, groups, film, act, p = case
+    t = gn_inputs(sum(map(ord, name)), shape, c0, c1, dtype, film)
+    dy = randn(5, *shape, c0 + c1, dtype=dtype)
+    kw = dict(act=act, p=p, rng=RNG if p else None)
+    want, bound = R.gn_act(t["x"], groups, t["weight"], t["bias"], film=t["film"], skip=t["skip"], dy=dy, **kw)
+    got = run_gn(t, groups, dy, **kw)
+    print(name, "worst ratio", R.check(got, want, bound, name))
+
+
+def test_one_value_a_group_has_no_gradient():
+    t = gn_inputs(3, (4, 1), 16, 0, torch.float32, "f32")
+    got = run_gn(t, 16, randn(1, 4, 1, 16), act="silu")
+    assert torch.equal(got["dx"], torch.zeros_like(got["dx"]))
+    assert torch.equal(got["dweight"], torch.zeros_like(got["dweight"]))
+
+
+@pytest.mark.parametrize("dtype", DTS, ids=["f32", "bf16", "f16"])
+def test_large_mean_keeps_its_variance(dtype):
+    """mean / deviation = 1000 (64 in the 16-bit types, whose steps would swallow the deviation): a sum of squares would lose it."""
+    off = 1000.0 if dtype == torch.float32 else 64.0
+    x = (randn(1, 2, 24, 24, 64) + off).to(dtype)
+    t = dict(x=x, skip=None, weight=torch.ones(64, device="cuda"), bias=torch.zeros(64, device="cuda"), film=None)
+    dy = randn(2, 2, 24, 24, 64, dtype=dtype)
+    want, bound = R.gn_act(x, 8, t["weight"], t["bias"], dy=dy)
+    R.check(run_gn(t, 8, dy), want, bound)
+
+
+@pytest.mark.parametrize("dtype", DTS, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("layout", ["channel_slice", "channel_slice_odd", "nchw", "channels_last", "misaligned", "row_slice", "expanded"])
+def test_strided_inputs(layout, dtype):
+    n, h, w, c, groups = 2, 10, 6, 48, 6
+    if layout == "channel_slice":
+        x = randn(1, n, h, w, 2 * c, dtype=dtype)[..., 16:16 + c]
+    elif layout == "channel_slice_odd":
+        x = randn(1, n, h, w, c + 5, dtype=dtype)[..., 3:3 + c]
+    elif layout == "nchw":
+        x = randn(1, n, c, h, w, dtype=dtype).permute(0, 2, 3, 1)
+    elif layout == "channels_last":
+        x = randn(1, n, c, h, w, dtype=dtype).to(memory_format=torch.channels_last).permute(0, 2, 3, 1)
+    elif layout == "misaligned":
+        x = randn(1, n * h * w * c + 1, dtype=dtype)[1:].view(n, h, w, c)
+    elif layout == "row_slice":
+        x = randn(1, n, h + 3, w + 2, c, dtype=dtype)[:, 1:h + 1, :w]
+    else:
+        x = randn(1, 1, h, w, c, dtype=dtype).expand(n, h, w, c)
+    film = randn(3, n, 3 * 2 * c + 1)[:, c:3 * c] * 0.3
+    t = dict(x=x, skip=None, weight=1 + randn(4, 2 * c)[::2] * 0.2, bias=randn(5, c) * 0.2, film=film)
+    dy = randn(6, n, c, h, w, dtype=dtype).permute(0, 2, 3, 1)
+    kw = dict(act="silu", p=0.2, rng=RNG)
+    want, bound = R.gn_act(t["x"], groups, t["weight"], t["bias"], film=film, dy=dy, **kw)
+    R.check(run_gn(t, groups, dy, **kw), want, bound, layout)
+
+
+def test_strided_skip_and_source_give_what_the_concatenation_gives():
+    base = randn(1, 2, 8, 8, 200, dtype=torch.bfloat16)
+    x, skip = base[..., :72], base[..., 80:136]
+    w, b = 1 + 0.1 * randn(2, 128), randn(3, 128)
+    cat = torch.cat([x, skip], -1)
+    a = F().group_norm_act(x, 16, w, b, skip=skip)
+    assert torch.equal(a, F().group_norm_act(cat, 16, w, b))
+    assert torch.equal(a, F().group_norm_act(x.contiguous(), 16, w, b, skip=skip.contiguous()))
+
+
+def test_non_finite_values_stay_in_their_group():
+    x = randn(1, 3, 6, 6, 32)
+    x[1, 2, 3, 5] = float("nan")
+    x[2, 0, 0, 31] = float("inf")
+    w, b = torch.ones(32, device="cuda"), torch.zeros(32, device="cuda")
+    dy = randn(2, 3, 6, 6, 32)
+    t = dict(x=x, skip=None, weight=w, bias=b, film=None)
+    got = run_gn(t, 4, dy)
+    bad = torch.zeros(3, 4, dtype=torch.bool)
+    bad[1, 0] = bad[2, 3] = True
+    for k in ("y", "dx"):
+        groups_bad = ~torch.isfinite(got[k].detach()).reshape(3, 36, 4, 8).all(3).all(1).cpu()
+        assert torch.equal(groups_bad, bad), k
+
+
+def test_extreme_activations_do_not_turn_into_nan():
+    """v = +-200: the exponential overflows, silu is v or 0 and its slope 1 or 0."""
+    x = randn(1, 2, 8, 8, 32)
+    t = dict(x=x, skip=None, weight=torch.ones(32, device="cuda"), bias=torch.tensor([200.0, -200.0] * 16, device="cuda"), film=None)
+    dy = randn(2, 2, 8, 8, 32)
+    want, bound = R.gn_act(x, 4, t["weight"], t["bias"], dy=dy)
+    R.check(run_gn(t, 4, dy), want, bound)
+
+
+@pytest.mark.parametrize("p", [0.0, 0.3])
+def test_gradients_against_differences(p):
+    """The loss sum(y * r) in 64-bit sums of fp32 results: a central difference of step 2^-6 along a random direction is off by the
+    rounding of y (bounded) / step plus step^2 / 6 times the third derivative; the direction is normalised, so both stay below
+    1e-3 of the gradients' norm here."""
+    n, h, w, c, g = 2, 6, 5, 32, 8
+    t = gn_inputs(7, (n, h, w), c, 0, torch.float32, "f32")
+    r = randn(9, n, h, w, c)
+    kw = dict(p=p, rng=RNG if p else None)
+    got = run_gn(t, g, r, **kw)
+    for i, k in enumerate(("x", "weight", "bias", "film")):
+        d = randn(20 + i, *t[k].shape)
+        d /= d.norm()
+        step = 2.0 ** -6
+        val = []
+        for s in (step, -step):
+            q = dict(t, **{k: t[k] + s * d})
+            y = F().group_norm_act(q["x"], g, q["weight"], q["bias"], film=q["film"], **kw)
+            val.append((y.double() * r.double()).sum().item())
+        fd = (val[0] - val[1]) / (2 * step)
+        an = (got["d" + k].double() * d.double()).sum().item()
+        assert abs(fd - an) <= 1e-3 * got["d" + k].double().norm().item(), (k, fd, an)
+
+
+def test_only_the_gradients_asked_for():
+    t = gn_inputs(8, (2, 4, 4), 32, 32, torch.float32, "f32")
+    skip = t["skip"].requires_grad_()
+    y = F().group_norm_act(t["x"], 8, t["weight"], t["bias"], film=t["film"], skip=skip)
+    y.sum().backward()
+    assert skip.grad.shape == skip.shape and t["x"].grad is None
+    with pytest.raises(RuntimeError):      # differentiable once
+        w = t["weight"].requires_grad_()
+        (gw,) = torch.autograd.grad(F().group_norm_act(t["x"], 8, w, t["bias"], skip=skip).sum(), w, create_graph=True)
+        gw.sum().backward()
+
+
+def test_repeatable_and_independent_of_the_batch():
+    t = gn_inputs(11, (24, 32, 32), 128, 0, torch.bfloat16, "f32")
+    dy = randn(12, 24, 32, 32, 128, dtype=torch.bfloat16)
+    a, b = run_gn(t, 32, dy), run_gn(t, 32, dy)
+    for k in a:
+        assert torch.equal(a[k], b[k]), k
+    one = {k: (v[5:6] if k in ("x", "film") else v) for k, v in t.items()}
+    c = run_gn(one, 32, dy[5:6])
+    for k in ("y", "dx", "dfilm", "stats"):
+        assert torch.equal(a[k][5:6], c[k]), k
+
+
+@pytest.mark.parametrize("dtype", DTS, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n", [1, 7, 8, 9, 63, 4096, 100003])
+@pytest.mark.parametrize("p", [0.0, 0.1, 0.5, 1.0])
+def test_dropout(n, p, dtype):
+    x = randn(n, n, dtype=dtype).requires_grad_()
+    dy = randn(n + 1, n, dtype=dtype)
+    y = F().dropout(x, p, RNG)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    f = R.drop_factor(n, p, RNG)
+    for got, src in ((y, x), (dx, dy)):
+        want = src.detach().double().cpu() * f
+        got = got.detach().double().cpu()
+        assert torch.equal(got == 0, want == 0)
+        # half a step of the type (below fp16's normal range steps are 2^-24 whatever the value), of the fp32 scale and product
+        assert bool(((got - want).abs() <= want.abs() * (R.HALF[dtype] * 1.001 + 2 * R.U) + R.TINY[dtype]).all())
+
+
+def test_dropout_draws_are_the_published_generator_at_far_indices():
+    """Element 2^32 + k of a tensor longer than 2^32: 64-bit indices all the way (8.6 GB in, 8.6 GB out)."""
+    n = (1 << 32) + 1027
+    x = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    y = F().dropout(x, 0.5, RNG)
+    for first, count in ((0, 64), ((1 << 32) - 64, 1024 + 67)):
+        want = R.draws(count, RNG, first) >= 32768
+        assert np.array_equal((y[first:first + count] != 0).cpu().numpy(), want)
+    del x, y
+    torch.cuda.empty_cache()
+
+
+def test_dropout_statistics_and_streams():
+    n = 1 << 22
+    x = torch.ones(n, device="cuda")
+    a = F().dropout(x, 0.1, (1, 2))
+    # kept ~ Binomial(n, 0.9): 6 deviations
+    assert abs((a != 0).double().mean().item() - (1 - 6554 / 65536)) < 6 * (0.09 / n) ** 0.5
+    assert abs(a.double().mean().item() - 1) < 6 * (0.09 / n) ** 0.5 / 0.9
+    for other in ((1, 3), (2, 2), (1 + (1 << 40), 2), (1, 2 + (1 << 35))):
+        b = F().dropout(x, 0.1, other)
+        both = ((a != 0) == (b != 0)).double().mean().item()        # independent: 0.81 + 0.01
+        assert abs(both - 0.82) < 6 * (0.82 * 0.18 / n) ** 0.5 + 1e-4
+    assert torch.equal(a, F().dropout(x, 0.1, (1, 2)))
+
+
+def test_dropout_layouts_and_non_finite_values():
+    x = randn(1, 40, 30)
+    f = R.drop_factor(1200, 0.3, RNG).reshape(40, 30)
+    y = F().dropout(x.t(), 0.3, RNG).cpu()
+    assert torch.equal(y == 0, R.drop_factor(1200, 0.3, RNG).reshape(30, 40) == 0)
+    v = randn(2, 1201)[1:].view(40, 30)
+    assert torch.equal(F().dropout(v, 0.3, RNG).cpu() == 0, f == 0)
+    z = torch.full((40, 30), float("nan"), device="cuda")
+    assert torch.equal(F().dropout(z, 0.3, RNG).cpu() == 0, f == 0)
+    assert F().dropout(torch.empty(0, 5, device="cuda"), 0.5, RNG).shape == (0, 5)
+
+
+def test_block_as_a_resblock_uses_it():
+    """norm -> FiLM -> SiLU -> dropout in one call = the norm without dropout followed by `dropout` with the same rng (fp32: the
+    scale multiplies the same fp32 value), forward and backward."""
+    t = gn_inputs(31, (3, 9, 5), 40, 0, torch.float32, "f32")
+    x = t["x"].requires_grad_()
+    dy = randn(2, 3, 9, 5, 40)
+    a = F().group_norm_act(x, 10, t["weight"], t["bias"], film=t["film"], p=0.2, rng=RNG)
+    b = F().dropout(F().group_norm_act(x, 10, t["weight"], t["bias"], film=t["film"]), 0.2, RNG)
+    assert torch.equal(a, b)
+    ga, gb = torch.autograd.grad(a, x, dy)[0], torch.autograd.grad(b, x, dy)[0]
+    assert torch.equal(ga, gb)
+
+
+def test_empty_inputs():
+    w, b = torch.ones(32, device="cuda").requires_grad_(), torch.zeros(32, device="cuda")
+    for shape in ((0, 4, 4, 32), (2, 0, 4, 32)):
+        x = torch.empty(shape, device="cuda").requires_grad_()
+        y = F().group_norm_act(x, 8, w, b)
+        assert y.shape == shape
+        gx, gw = torch.autograd.grad(y, [x, w], torch.empty(shape, device="cuda"))
+        assert gx.shape == shape and torch.equal(gw, torch.zeros_like(gw))
+
+
+def test_on_another_stream():
+    t = gn_inputs(41, (8, 32, 32), 256, 0, torch.bfloat16, "f32")
+    dy = randn(3, 8, 32, 32, 256, dtype=torch.bfloat16)
+    ref = run_gn(t, 32, dy, p=0.1, rng=RNG)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = run_gn(t, 32, dy, p=0.1, rng=RNG)
+    s.synchronize()
+    for k in ref:
+        assert torch.equal(ref[k], got[k]), k
+
+
+def test_two_streams_at_once():
+    ts = [gn_inputs(50 + i, (16, 64, 64), 128, 0, torch.bfloat16, "f32") for i in range(2)]
+    dys = [randn(60 + i, 16, 64, 64, 128, dtype=torch.bfloat16) for i in range(2)]
+    refs = [run_gn(t, 32, dy) for t, dy in zip(ts, dys)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run_gn(ts[i], 32, dys[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            for k in refs[i]:
+                assert torch.equal(refs[i][k], g[k]), (i, k)
+
+
+def test_captured_step_replays_with_new_inputs_and_new_draws():
+    """Forward and backward by hand in one graph, the draws from a device rng; every replay equals the eager result, with eager
+    work of the same operators between the replays."""
+    f = F()
+    t = gn_inputs(71, (4, 64, 64), 64, 0, torch.bfloat16, "f32")
+    dy = randn(72, 4, 64, 64, 64, dtype=torch.bfloat16)
+    rng = torch.tensor([5, 6], device="cuda")
+    args = (32, t["weight"], t["bias"])
+
+    def step():
+        y, stats = f.group_norm_act_forward(t["x"], *args, film=t["film"], p=0.1, rng=rng)
+        z = f.dropout(y, 0.2, rng)
+        dz = f.dropout(dy, 0.2, rng)
+        return (y, z) + f.group_norm_act_backward(dz, stats, t["x"], *args, film=t["film"], p=0.1, rng=rng)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    seen = []
+    for i in range(5):
+        t["x"].copy_(randn(80 + i, 4, 64, 64, 64))
+        rng.copy_(torch.tensor([5 + i, 6]))
+        graph.replay()
+        got = [o.clone() for o in out if o is not None]
+        want = [o for o in step() if o is not None]
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), i
+        seen.append(got[1] == 0)
+    assert not torch.equal(seen[0], seen[1])
+
+
+def test_two_graphs_replayed_at_once():
+    f = F()
+    ts = [gn_inputs(90 + i, (8, 64, 64), 128, 0, torch.bfloat16, "f32") for i in range(2)]
+    dys = [randn(95 + i, 8, 64, 64, 128, dtype=torch.bfloat16) for i in range(2)]
+    graphs, outs, wants = [], [], []
+    for t, dy in zip(ts, dys):
+        def step(t=t, dy=dy):
+            y, stats = f.group_norm_act_forward(t["x"], 32, t["weight"], t["bias"], film=t["film"])
+            return (y,) + f.group_norm_act_backward(dy, stats, t["x"], 32, t["weight"], t["bias"], film=t["film"])
+        wants.append([o.clone() for o in step() if o is not None])
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step())
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, wants):
+            for a, b in zip([q for q in o if q is not None], w):
+                assert torch.equal(a, b)
+
+
+def test_autograd_through_leaves_is_refused_under_capture():
+    from ivid_amd._lib import IvidHipError
+    x = randn(1, 2, 4, 4, 32).requires_grad_()
+    w, b = torch.ones(32, device="cuda"), torch.zeros(32, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    refused = []
+    with torch.cuda.graph(g):
+        for fn in (lambda: F().group_norm_act(x, 8, w, b), lambda: F().dropout(x, 0.5, RNG)):
+            try:
+                fn()
+            except IvidHipError as e:
+                refused.append(str(e))
+        keep = w + 1  # noqa: F841  (a graph with a node)
+    assert len(refused) == 2
+    assert F().group_norm_act(x, 8, w, b).requires_grad
+
+
+def test_a_rewritten_rng_tensor_is_noticed():
+    x = randn(1, 100).requires_grad_()
+    rng = torch.tensor([1, 2], device="cuda")
+    y = F().dropout(x, 0.5, rng)
+    rng.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", DTS, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape,c0,c1,groups", [((3, 7, 5), 24, 0, 6), ((2, 33), 50, 14, 8), ((2, 40, 41), 64, 0, 32), ((1, 70, 70), 72, 0, 9)])
+def test_nothing_is_written_outside_the_outputs(shape, c0, c1, groups, dtype):
+    """Every output and the scratch sit between guard bytes."""
+    import ctypes
+    from ivid_amd import _lib
+    f = F()
+    t = gn_inputs(101, shape, c0, c1, dtype, "same")
+    c = c0 + c1
+    call = f._Call(t["x"], groups, t["weight"], t["bias"], t["film"], t["skip"], "silu", 1e-5, 0.1, RNG)
+    pix = t["x"].numel() // c0
+    esz = t["x"].element_size()
+    guarded = []
+
+    def buf(nbytes):
+        b = torch.full((nbytes + 512,), 0xA5, dtype=torch.uint8, device="cuda")
+        guarded.append((b, nbytes))
+        return b.data_ptr() + 256
+    lib = _lib.load()
+    st = torch.cuda.current_stream().cuda_stream
+    nb = [lib.ivid_gn_act_scratch_bytes(ctypes.byref(call.desc), i) for i in range(2)]
+    stats = buf(shape[0] * groups * 8)
+    _lib.call("ivid_gn_act_forward", ctypes.byref(call.desc), buf(pix * c * esz), stats, buf(nb[0]), nb[0], st)
+    dy = randn(7, *shape, c, dtype=dtype)
+    _lib.call("ivid_gn_act_backward", ctypes.byref(call.desc), stats, dy.data_ptr(), buf(pix * c0 * esz), buf(pix * c1 * esz) if c1 else None,
+              buf(4 * c), buf(4 * c), buf(shape[0] * 2 * c * esz), buf(nb[1]), nb[1], st)
+    n = pix * c + 3
+    x = randn(8, n, dtype=dtype)
+    _lib.call("ivid_dropout", f._DTYPES[dtype], x.data_ptr(), buf(n * esz), n, 0.5, 1, 2, None, st)
+    torch.cuda.synchronize()
+    for b, nbytes in guarded:
+        assert bool((b[:256] == 0xA5).all()) and bool((b[256 + nbytes:] == 0xA5).all())
