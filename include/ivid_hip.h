@@ -285,7 +285,8 @@ int ivid_gn_apply_p(int dtype, const void* src0, const void* src0_lo, int C0, co
  *   y = drop(act(u * (1 + scale) + shift)),  u = xhat * gamma + beta,  xhat = (x - mean) * rstd
  * x = cat[src0, src1] over channels, N samples of HW pixels; mean and biased variance per (sample, group) in fp32 or wider;
  * act 0 none, 1 SiLU; drop as in ivid_dropout, element index = row-major index in the [N,HW,C0+C1] output.
- * Any HW >= 1, any C0 + C1 divisible by groups, any element alignment. */
+ * Any N, HW >= 1, any C0 + C1 divisible by groups; src0, src1, gamma, beta and film may be aligned to an element only, every other
+ * pointer of a tensor to 16 bytes. */
 typedef struct {
   int dtype;                              /* IVID_F32, IVID_BF16 or IVID_F16: src, out, dy, dsrc */
   int N, HW, C0, C1, groups, act;         /* C1 = 0 and src1 = NULL: one source */
@@ -297,8 +298,10 @@ typedef struct {
   double eps, p;                          /* p = 0: no dropout */
   unsigned long long seed, stream_id;     /* of the dropout draws */
   const unsigned long long* rng;          /* NULL, or device {seed, stream_id}: replaces the two above, read when the kernel runs */
+  int max_polls;                          /* 0: the library's bound on a workgroup's wait for its sample's other sums; results never
+                                           * depend on it (a workgroup that stops waiting computes what is missing itself) */
 } ivid_gn_act_desc;
-/* Device scratch of one call in bytes (8-byte aligned), -1 for a malformed descriptor.  Contents need not be kept between calls,
+/* Device scratch of one call in bytes (16-byte aligned), -1 for a malformed descriptor.  Contents need not be kept between calls,
  * nor between a forward and its backward; two calls that may run at once need a scratch each. */
 long long ivid_gn_act_scratch_bytes(const ivid_gn_act_desc* host_desc, int backward);
 /* out [N,HW,C0+C1]; stats fp32 [N,groups,2] = mean, rstd (what the backward pass needs) */

@@ -91,7 +91,7 @@ class GnActDesc(C.Structure):       # ivid_gn_act_desc
                    ("src1", C.c_void_p), ("ld1", C.c_longlong), ("sn1", C.c_longlong),
                    ("gamma", C.c_void_p), ("beta", C.c_void_p), ("film", C.c_void_p), ("film_dtype", C.c_int),
                    ("film_ld", C.c_longlong), ("eps", C.c_double), ("p", C.c_double), ("seed", C.c_ulonglong),
-                   ("stream_id", C.c_ulonglong), ("rng", C.c_void_p)])
+                   ("stream_id", C.c_ulonglong), ("rng", C.c_void_p), ("max_polls", C.c_int)])
 
 
 SAMPLE_DDIM, SAMPLE_DDPM = 0, 1

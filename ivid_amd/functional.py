@@ -25,6 +25,7 @@ from . import _lib
 
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _ACTS = {"none": 0, "silu": 1}
+_MAX_POLLS = 0      # ivid_gn_act_desc.max_polls; the tests lower it
 
 
 def _rng_args(rng, p, device):
@@ -200,7 +201,8 @@ class _Call:
         self.desc = _lib.GnActDesc(
             _DTYPES[x.dtype], n, 0 if self.empty else x.numel() // (n * c0), c0, c1, groups, _ACTS[act],
             x.data_ptr(), ld0, sn0, ptr(skip), ld1, sn1, weight.data_ptr(), bias.data_ptr(), ptr(film),
-            _DTYPES[film.dtype] if film is not None else 0, film.stride(0) if film is not None else 0, eps, p, seed, sid, rng_ptr)
+            _DTYPES[film.dtype] if film is not None else 0, film.stride(0) if film is not None else 0, eps, p, seed, sid, rng_ptr,
+            _MAX_POLLS)
 
     def scratch(self, backward):
         nbytes = _lib.load().ivid_gn_act_scratch_bytes(C.byref(self.desc), backward)
@@ -225,6 +227,8 @@ class _Call:
         if stats.shape != (self.n, self.groups, 2) or stats.dtype != torch.float32 or stats.device != self.device:
             raise ValueError("stats must be what the forward call returned")
         dy, stats = dy.contiguous(), stats.contiguous()
+        if dy.data_ptr() % 16:
+            dy = dy.clone()
         new = torch.zeros if self.empty else torch.empty
         dev = self.device
         dx = new(self.shape[:-1] + (self.c0,), dtype=self.dtype, device=dev)

@@ -441,3 +441,36 @@ def test_nothing_is_written_outside_the_outputs(shape, c0, c1, groups, dtype):
     torch.cuda.synchronize()
     for b, nbytes in guarded:
         assert bool((b[:256] == 0xA5).all()) and bool((b[256 + nbytes:] == 0xA5).all())
+
+
+@pytest.mark.parametrize("dtype", DTS, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape,c0,c1,groups", [((3, 64, 64), 128, 0, 32), ((2, 61, 67), 50, 0, 10), ((2, 50, 50), 1000, 24, 1), ((1, 128, 128), 33, 0, 3)])
+def test_a_workgroup_that_stops_waiting_changes_nothing(shape, c0, c1, groups, dtype, monkeypatch):
+    """One poll: workgroups compute the sums that have not come yet themselves; every output is the same bit for bit."""
+    t = gn_inputs(111, shape, c0, c1, dtype, "f32")
+    dy = randn(112, *shape, c0 + c1, dtype=dtype)
+    ref = run_gn(t, groups, dy, p=0.1, rng=RNG)
+    monkeypatch.setattr(F(), "_MAX_POLLS", 1)
+    for _ in range(3):
+        got = run_gn(t, groups, dy, p=0.1, rng=RNG)
+        for k in ref:
+            assert torch.equal(ref[k], got[k]), k
+    want, bound = R.gn_act(t["x"], groups, t["weight"], t["bias"], film=t["film"], skip=t["skip"], dy=dy, p=0.1, rng=RNG)
+    R.check(ref, want, bound)
+
+
+def test_offsets_beyond_32_bits():
+    """6.4e9 values in one call (12.9 GB a tensor): the last sample equals the call on it alone."""
+    n, hw, c = 3, 1 << 24, 128
+    x = torch.empty(n, hw, c, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(1))
+    w, b = 1 + 0.1 * randn(2, c), randn(3, c)
+    y, stats = F().group_norm_act_forward(x, 32, w, b)
+    y1, stats1 = F().group_norm_act_forward(x[2:], 32, w, b)
+    assert torch.equal(y[2:], y1) and torch.equal(stats[2:], stats1)
+    assert abs(stats[..., 0].abs().max().item()) < 1e-3 and (stats[..., 1] - 1).abs().max().item() < 1e-3
+    del y1
+    dx = F().group_norm_act_backward(x, stats, x, 32, w, b)[0]
+    dx1 = F().group_norm_act_backward(x[2:], stats1, x[2:], 32, w, b)[0]
+    assert torch.equal(dx[2:], dx1)
+    del x, y, dx, dx1
+    torch.cuda.empty_cache()
