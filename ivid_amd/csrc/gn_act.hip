@@ -12,11 +12,11 @@
 //   * a sum is published as one 64-bit word {value, 1} by a relaxed agent-scope store: value and arrival in one, no fences.  The words
 //     are zeroed by a launch in front (none for K = 1);
 //   * every workgroup of the cluster adds the K partial sums itself, in the same order, in 64 bits: equal results, no atomics;
-//   * a wait ends after a bounded number of polls: the workgroup then computes the missing tile's sums itself -- by the same code, so
-//     bit for bit the same -- publishes them and goes on.  No workgroup depends on another one being resident.
+//   * a wait ends after a bounded number of polls: the workgroup then computes the missing tile's sums itself, in the same order and
+//     so bit for bit the same, publishes them and goes on.  No workgroup depends on another one being resident.
 // A cluster of more than MAX_K tiles would not be resident at once: it takes two launches, sums and results (PH_SUMS, PH_RESULT), with
 // a small one between them that adds the words, and reads its inputs twice.
-// Sums inside a tile are two-pass (mean, then centred squares) over the registers: a large mean costs no digits.
+// Squares are centred on the tile's own means: a large mean costs no digits.
 #include <math.h>
 #include <utility>
 #include "common.h"
@@ -25,10 +25,13 @@
 
 int ivid_drop_rng(double p, unsigned long long seed, unsigned long long stream_id, const unsigned long long* rng, DropRng* out);
 
+#pragma clang fp contract(off)      // every fused multiply-add below is written out: a sum has the same bits wherever it is computed
+
 namespace {
-constexpr int NT = 256;
-constexpr int MAX_GS = 64;        // groups of a slab: one of the 256 threads' 4-lane teams each
-constexpr int MAX_POLLS = 512;    // ~ 0.3 ms
+constexpr int NT_FWD = 512, NT_BWD = 256, NT_AUX = 256;
+constexpr int MAX_GS = 64;        // groups of a slab: at least four lanes each in the reductions
+constexpr int MAX_COL = 1024;     // channels of a tile
+constexpr int MAX_POLLS = 512;    // ~ 1 ms
 constexpr int MAX_K = 128;        // tiles of a cluster that runs as one launch
 enum { PH_ALL = 0, PH_SUMS = 1, PH_RESULT = 2 };
 
@@ -63,23 +66,40 @@ __device__ __forceinline__ typename Piece<T, VE>::mem pack(const float* f) {
     return __builtin_bit_cast(typename Piece<T, VE>::mem, v);
   }
 }
-// The compiler must not carry a piece's fp32 values from one pass over the registers to the next: they would need twice the registers.
+// The compiler must not carry a piece's fp32 values, or the counts that tell which pieces there are, from one pass over the registers to
+// the next: they would need more registers than the data.
 template <typename R>
 __device__ __forceinline__ void forget(R& v) { asm volatile("" : "+v"(v)); }
 
-// f(0), f(1), ... f(N - 1) as straight-line code: the sweeps of a tile live in registers, which cannot be indexed by a loop
+// threadIdx.x as a value of its own: what is computed from it is not shared with, and so not kept for, another part of the kernel
+__device__ __forceinline__ int fresh_thread() {
+  int t = threadIdx.x;
+  forget(t);
+  return t;
+}
+
+// f(0), f(1), ... f(N - 1) as straight-line code: the sweeps of a tile live in registers, which cannot be indexed by a loop.  No branch
+// around them either: the loads have to be unconditional for the compiler to wait for one after the other.
 template <typename F, int... I>
-__device__ __forceinline__ void sweeps_of(F&& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+__device__ __forceinline__ void sweeps_of(F& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
 template <int N, typename F>
-__device__ __forceinline__ void sweeps(F&& f) { sweeps_of(f, std::make_integer_sequence<int, N>{}); }
+__device__ __forceinline__ void sweeps(F f) { sweeps_of(f, std::make_integer_sequence<int, N>{}); }
+
+// n / d for n < 2^24 as a multiplication: the kernels divide by run-time sizes in front of their first load
+struct Div {
+  uint32_t d, m, s;
+  __device__ __forceinline__ int of(int n) const { return (int)(((uint64_t)(uint32_t)n * m) >> s); }
+};
 
 // How the work is cut (see cut_up()); part of the kernel arguments.
 struct Cut {
   int S, nslab;             // channels of a slab (a multiple of the group and of the piece), slabs of a sample
   int PP, kcols;            // pieces of a tile's row; column chunks of a slab (1 unless a slab's row is wider than the workgroup)
   int RPI, nv, rows, krows; // pixels per sweep of the workgroup, sweeps, pixels of a tile, tiles down a sample
-  int K, GS, W;             // tiles of a cluster, groups of a slab, lanes per group in the reductions (a power of two)
+  int K, GS, logW;          // tiles of a cluster, groups of a slab, log2 of the lanes per group (a team) in the reductions
+  int seg, logseg;          // channels of a run: the largest power of two that divides the group and the piece
   int polls, phase;
+  Div by_nslab, by_K, by_PP, by_Cg, by_runs;
 };
 
 struct GnArgs {
@@ -100,12 +120,6 @@ __device__ __forceinline__ float film_at(const GnArgs& a, long long i) {
   return a.film_kind == 1 ? ((const float*)a.film)[i] : (float)((const T*)a.film)[i];
 }
 
-// a * b rounded: not contracted into a following addition (with one value a group, g - sum(g) / M has to cancel exactly)
-__device__ __forceinline__ float mul_rounded(float a, float b) {
-#pragma clang fp contract(off)
-  return a * b;
-}
-
 __device__ __forceinline__ void publish(unsigned long long* w, float v) {
   __hip_atomic_store(w, (1ull << 32) | __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
@@ -115,28 +129,34 @@ __device__ __forceinline__ unsigned long long peek(const unsigned long long* w) 
 
 // One tile as a thread sees it.
 struct Tile {
-  int row0, nrow;      // first pixel, pixels
+  int kc, row0, nrow;  // column chunk, first pixel, pixels
   int cb, ce;          // channels [cb, ce)
   int r0, piece, c;    // this thread's first row, piece and channel
-  bool active;
+  int mine;            // its rows are r0, r0 + RPI, ... while this, less RPI a sweep, stays positive; 0: it has none
 };
 template <int VE>
-__device__ __forceinline__ Tile tile_of(const GnArgs& a, int slab, int k) {
+__device__ __forceinline__ Tile tile_of(const GnArgs& a, int slab, int k, int thread) {
   const Cut& q = a.cut;
-  const int kr = q.kcols == 1 ? k : k / q.kcols, kc = q.kcols == 1 ? 0 : k - kr * q.kcols;
   Tile t;
+  int kr = k;
+  t.kc = 0;
+  if (q.kcols > 1) {
+    kr = k / q.kcols;
+    t.kc = k - kr * q.kcols;
+  }
   const int cs = slab * q.S, cend = min(cs + q.S, a.C);
-  t.cb = cs + kc * q.PP * VE;
+  t.cb = cs + t.kc * q.PP * VE;
   t.ce = min(t.cb + q.PP * VE, cend);
   t.row0 = kr * q.rows;
   t.nrow = min(q.rows, a.HW - t.row0);
-  t.r0 = threadIdx.x / q.PP;
-  t.piece = threadIdx.x - t.r0 * q.PP;
+  t.r0 = q.by_PP.of(thread);
+  t.piece = thread - t.r0 * q.PP;
   t.c = t.cb + t.piece * VE;
-  t.active = t.r0 < q.RPI && t.c < t.ce;
+  const bool active = t.r0 < q.RPI && t.c < t.ce;
+  t.mine = active ? t.nrow - t.r0 : 0;
   return t;
 }
-// values of group g (of the slab) in tile k
+// channels of group g (of the slab) in column chunk kc
 __device__ __forceinline__ int columns_of(const GnArgs& a, int slab, int kc, int g, int VE) {
   const int cs = slab * a.cut.S;
   const int cb = cs + kc * a.cut.PP * VE, ce = min(cb + a.cut.PP * VE, min(cs + a.cut.S, a.C));
@@ -145,73 +165,79 @@ __device__ __forceinline__ int columns_of(const GnArgs& a, int slab, int kc, int
 }
 __device__ __forceinline__ int groups_of(const GnArgs& a, int slab) { return min(a.cut.GS, a.G - slab * a.cut.GS); }
 
-// per-thread channel sums s[VE] -> group sums of the tile in gs[] (LDS), the same order for every workgroup
-template <int VE>
-__device__ __forceinline__ void reduce_groups(const GnArgs& a, const Tile& t, int slab, const float* s, float* red, float* gs) {
-  const Cut& q = a.cut;
-  const int RS = q.PP * VE + 8;     // padded rows: the lanes of a team read several rows at once
-  if (t.r0 < q.RPI) {
-#pragma unroll
-    for (int e = 0; e < VE; ++e) red[t.r0 * RS + t.piece * VE + e] = s[e];
+// Where a thread's first piece is; rows it does not have are read from the tile's last one (unconditional loads: all in flight at once).
+template <typename T, int VE>
+struct Source {
+  const char* p;
+  long long step;
+  __device__ __forceinline__ Source(const GnArgs& a, int n, const Tile& t) {
+    const int c = t.c < t.ce ? t.c : t.cb;
+    const bool second = c >= a.C0;
+    const long long ld = second ? a.ld1 : a.ld0, sn = second ? a.sn1 : a.sn0;
+    step = ld * (a.cut.RPI * (int)sizeof(T));
+    p = (second ? a.src1 : a.src0) + ((long long)n * sn + (long long)(t.row0 + min(t.r0, t.nrow - 1)) * ld + (c - (second ? a.C0 : 0))) * (long long)sizeof(T);
   }
-  __syncthreads();
-  const int g = threadIdx.x / q.W, l = threadIdx.x - g * q.W;
-  const int c0 = slab * q.S + g * a.Cg;
-  const int lo = max(c0, t.cb), hi = min(c0 + a.Cg, t.ce), w = hi - lo;
-  float sum = 0.f;
-  if (g < groups_of(a, slab) && w > 0) {
-    const int dr = q.W / w, dj = q.W - dr * w;
-    int row = l / w, j = l - row * w;
-    while (row < q.RPI) {
-      sum += red[row * RS + lo - t.cb + j];
-      row += dr;
-      j += dj;
-      if (j >= w) { j -= w; ++row; }
-    }
-  }
-  for (int o = q.W >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-  if (l == 0 && g < q.GS) gs[g] = sum;
-  __syncthreads();
-}
+};
 
-// The cluster's words of this (sample, slab): [K][GS][2].  Adds them per group, in 64 bits, in a fixed order: weight(k, g) * first [+
-// second + weight * first^2 for the forward pass].  Returns the first tile whose words have not come, or -1 with the sums in out[].
+// The cluster's words of this (sample, slab): [K][GS][2].  Adds them per group, in 64 bits, in a fixed order: for the forward pass
+// (MOMENTS) count * mean and squares + count * mean^2.  Returns the first tile whose words have not come, or -1 with the sums in out[].
 template <int VE, bool MOMENTS>
 __device__ __forceinline__ int gather(const GnArgs& a, int slab, const unsigned long long* words, int* missing, double2* out) {
   const Cut& q = a.cut;
-  const int g = threadIdx.x / q.W, l = threadIdx.x - g * q.W;
-  if (threadIdx.x == 0) *missing = 0x7fffffff;
+  const int thread = fresh_thread();
+  const int g = thread >> q.logW, W = 1 << q.logW, l = thread & (W - 1);
+  if (thread == 0) *missing = 0x7fffffff;
   __syncthreads();
   double s1 = 0.0, s2 = 0.0;
   if (g < groups_of(a, slab)) {
-    for (int k = l; k < q.K; k += q.W) {
-      const int kr = q.kcols == 1 ? k : k / q.kcols, kc = q.kcols == 1 ? 0 : k - kr * q.kcols;
-      const unsigned long long* w = words + ((size_t)k * q.GS + g) * 2;
-      unsigned long long w0, w1;
-      bool there = false;
+    constexpr int U = 2;      // tiles asked for at once
+#pragma unroll 1
+    for (int k0 = l; k0 < q.K; k0 += U * W) {
+      unsigned long long w0[U], w1[U];
+      int miss = 0;
       for (int i = 0; i < q.polls; ++i) {
-        w0 = peek(w);
-        w1 = peek(w + 1);
-        there = (w0 >> 32) && (w1 >> 32);
-        if (there) break;
-        __builtin_amdgcn_s_sleep(4);
+        miss = 0x7fffffff;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (k0 + u * W < q.K) {
+            const unsigned long long* w = words + ((size_t)(k0 + u * W) * q.GS + g) * 2;
+            w0[u] = peek(w);
+            w1[u] = peek(w + 1);
+          }
+        }
+#pragma unroll
+        for (int u = U - 1; u >= 0; --u)
+          if (k0 + u * W < q.K && !((w0[u] >> 32) && (w1[u] >> 32))) miss = k0 + u * W;
+        if (miss == 0x7fffffff) break;
+        __builtin_amdgcn_s_sleep(1);
       }
-      if (!there) {
-        atomicMin(missing, k);
+      if (miss != 0x7fffffff) {
+        atomicMin(missing, miss);
         break;
       }
-      const double x0 = (double)__uint_as_float((unsigned)w0), x1 = (double)__uint_as_float((unsigned)w1);
-      if constexpr (MOMENTS) {
-        const double cnt = (double)min(q.rows, a.HW - kr * q.rows) * (double)columns_of(a, slab, kc, g, VE);
-        s1 += cnt * x0;
-        s2 += x1 + cnt * x0 * x0;
-      } else {
-        s1 += x0;
-        s2 += x1;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + u * W;
+        if (k < q.K) {
+          const double x0 = (double)__uint_as_float((unsigned)w0[u]), x1 = (double)__uint_as_float((unsigned)w1[u]);
+          if constexpr (MOMENTS) {
+            int kr = k, kc = 0;
+            if (q.kcols > 1) {
+              kr = k / q.kcols;
+              kc = k - kr * q.kcols;
+            }
+            const double cnt = (double)min(q.rows, a.HW - kr * q.rows) * (double)columns_of(a, slab, kc, g, VE);
+            s1 += cnt * x0;
+            s2 += x1 + cnt * x0 * x0;
+          } else {
+            s1 += x0;
+            s2 += x1;
+          }
+        }
       }
     }
   }
-  for (int o = q.W >> 1; o > 0; o >>= 1) {
+  for (int o = W >> 1; o > 0; o >>= 1) {
     s1 += __shfl_xor(s1, o);
     s2 += __shfl_xor(s2, o);
   }
@@ -222,70 +248,199 @@ __device__ __forceinline__ int gather(const GnArgs& a, int slab, const unsigned 
   return m == 0x7fffffff ? -1 : m;
 }
 
-// gamma * (1 + s) and beta * (1 + s) + t of one channel
+// gamma * (1 + s) and beta * (1 + s) + t of one channel, in two steps: the loads are issued in front of the tile's (they come back in
+// order: behind them they would be waited for together with the whole tile), the arithmetic is done later
 template <typename T>
-__device__ __forceinline__ float2 affine(const GnArgs& a, int n, int c) {
-  float w = a.gamma[c], b = a.beta[c];
-  if (a.film_kind) {
-    const float gain = 1.0f + film_at<T>(a, (long long)n * a.film_ld + c);
-    w *= gain;
-    b = b * gain + film_at<T>(a, (long long)n * a.film_ld + a.C + c);
+struct Affine {
+  float w, b;
+  uint32_t s, t;      // as stored
+  __device__ __forceinline__ void load(const GnArgs& a, int n, int c) {
+    w = a.gamma[c];
+    b = a.beta[c];
+    s = t = 0;
+    const long long i = (long long)n * a.film_ld + c;
+    if (a.film_kind == 1) {
+      s = ((const uint32_t*)a.film)[i];
+      t = ((const uint32_t*)a.film)[i + a.C];
+    } else if (a.film_kind == 2) {
+      s = ((const typename Piece<T, 1>::mem*)a.film)[i];
+      t = ((const typename Piece<T, 1>::mem*)a.film)[i + a.C];
+    }
   }
-  return make_float2(w, b);
+  __device__ __forceinline__ float2 get(int film_kind) const {
+    typedef typename Piece<T, 1>::mem mem_t;
+    const float gain = 1.0f + (film_kind == 2 ? (float)__builtin_bit_cast(T, (mem_t)s) : __uint_as_float(s));
+    const float shift = film_kind == 2 ? (float)__builtin_bit_cast(T, (mem_t)t) : __uint_as_float(t);
+    return make_float2(w * gain, __builtin_fmaf(b, gain, shift));
+  }
+};
+// that of the thread's own first channel of the tile (channel threadIdx.x; any other one's where there is none)
+template <typename T>
+__device__ __forceinline__ Affine<T> first_affine(const GnArgs& a, int n, const Tile& t) {
+  Affine<T> f;
+  f.load(a, n, t.cb + min((int)threadIdx.x, t.ce - t.cb - 1));
+  return f;
 }
 template <int VE>
 __device__ __forceinline__ void read_channels(const float* ch, int piece, float* f) {
 #pragma unroll
   for (int e = 0; e < VE; ++e) f[e] = ch[piece * VE + e];
 }
-
-template <typename T, int VE>
-__device__ __forceinline__ const char* source(const GnArgs& a, int n, const Tile& t, long long& step) {
-  const bool second = t.c >= a.C0;
-  const long long ld = second ? a.ld1 : a.ld0, sn = second ? a.sn1 : a.sn0;
-  step = ld * a.cut.RPI * (long long)sizeof(T);
-  return (second ? a.src1 : a.src0) + ((long long)n * sn + (long long)(t.row0 + t.r0) * ld + (t.c - (second ? a.C0 : 0))) * (long long)sizeof(T);
+// f(j, coefficients) for this thread's channels of the tile; `first` = those of channel threadIdx.x, loaded long before
+template <int NT, typename T, typename F>
+__device__ __forceinline__ void each_channel(const GnArgs& a, int n, const Tile& t, const Affine<T>& first, F f) {
+  const int ncol = t.ce - t.cb;
+  if ((int)threadIdx.x < ncol) f((int)threadIdx.x, first.get(a.film_kind));
+  for (int j = threadIdx.x + NT; j < ncol; j += NT) {
+    Affine<T> other;
+    other.load(a, n, t.cb + j);
+    f(j, other.get(a.film_kind));
+  }
 }
 
-template <typename T, int VE, int NV>
+// ---- forward ----
+// v[] over the channels of a piece -> its sums over runs of q.seg channels (each inside one group), at every q.seg-th place
+template <int VE>
+__device__ __forceinline__ void add_runs(const Cut& q, float* v) {
+  if constexpr (VE >= 2) {
+    if (q.seg >= 2) {
+#pragma unroll
+      for (int e = 0; e < VE; e += 2) v[e] += v[e + 1];
+    }
+  }
+  if constexpr (VE >= 4) {
+    if (q.seg >= 4) {
+#pragma unroll
+      for (int e = 0; e < VE; e += 4) v[e] += v[e + 2];
+    }
+  }
+  if constexpr (VE >= 8) {
+    if (q.seg >= 8) v[0] += v[4];
+  }
+}
+// Sum over the tile of one value a channel and thread, per group: gs[g] (LDS), the same order for every workgroup.  A run is one word in
+// LDS; a team of W lanes adds its group's.
+template <int VE>
+__device__ __forceinline__ void group_sums(const GnArgs& a, const Tile& t, int slab, float* v, float* red, float* gs) {
+  const Cut& q = a.cut;
+  const int thread = fresh_thread();
+  add_runs<VE>(q, v);
+  const int RS = q.PP * (VE >> q.logseg);      // runs of a row
+  if (thread < q.RPI * q.PP) {
+    const int first = (thread * VE) >> q.logseg;      // a thread's runs follow those of the thread in front
+#pragma unroll
+    for (int e = 0; e < VE; ++e)
+      if ((e & (q.seg - 1)) == 0) red[first + (e >> q.logseg)] = v[e];
+  }
+  __syncthreads();
+  const int g = thread >> q.logW, W = 1 << q.logW, l = thread & (W - 1);
+  const int c0 = slab * q.S + g * a.Cg;
+  const int lo = (max(c0, t.cb) - t.cb) >> q.logseg, hi = g < groups_of(a, slab) ? (min(c0 + a.Cg, t.ce) - t.cb) >> q.logseg : 0;
+  const int w = max(hi - lo, 0), rows = min(q.RPI, t.nrow);
+  float sum = 0.f;
+  if (w > 0) {
+    const bool whole = w == a.Cg >> q.logseg;
+    const int dr = whole ? q.by_runs.of(W) : W / w, dj = W - dr * w;
+    int row = whole ? q.by_runs.of(l) : l / w;
+    int j = l - row * w;
+    while (row < rows) {
+      sum += red[row * RS + lo + j];
+      row += dr;
+      j += dj;
+      if (j >= w) { j -= w; ++row; }
+    }
+  }
+  for (int o = W >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  if (l == 0 && g < q.GS) gs[g] = sum;
+  __syncthreads();
+}
+
+// A thread's channel sums s[] -> the means of the tile's groups in gmean[] (LDS) and, of each of the thread's channels, in m[].
+template <int VE>
+__device__ __forceinline__ void tile_means(const GnArgs& a, const Tile& t, int slab, float* s, float* m, float* red, float* gmean) {
+  const Cut& q = a.cut;
+  group_sums<VE>(a, t, slab, s, red, gmean);
+  const int g = fresh_thread();
+  if (g < groups_of(a, slab)) gmean[g] /= fmaxf((float)t.nrow * (float)columns_of(a, slab, t.kc, g, VE), 1.f);
+  __syncthreads();
+  const int c = min(t.c, t.ce - 1);
+  int ge = q.by_Cg.of(c), r = c - ge * a.Cg;
+  ge -= slab * q.GS;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    m[e] = gmean[min(ge, MAX_GS - 1)];
+    if (++r == a.Cg) { r = 0; ++ge; }
+  }
+}
+
+// The sums of a tile that another workgroup holds, by streaming over it (gather() did not find them): the same operations in the
+// same order as in the kernel.
+template <typename T, int VE>
+__device__ __forceinline__ void help_forward(const GnArgs& a, int n, int slab, int k, float* red, float* gmean, float* gsq) {
+  const Tile t = tile_of<VE>(a, slab, k, fresh_thread());
+  float s[VE], m[VE];
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) s[e] = 0.f;
+    Source<T, VE> src(a, n, t);
+#pragma unroll 1
+    for (int left = t.mine; left > 0; left -= a.cut.RPI) {
+      float f[VE];
+      unpack<T, VE>(*(const typename Piece<T, VE>::mem*)src.p, f);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        if (pass == 0) s[e] += f[e];
+        else { const float d = f[e] - m[e]; s[e] = __builtin_fmaf(d, d, s[e]); }
+      }
+      src.p += src.step;
+    }
+    if (pass == 0) tile_means<VE>(a, t, slab, s, m, red, gmean);
+  }
+  group_sums<VE>(a, t, slab, s, red, gsq);
+}
+
+template <int NT, typename T, int VE, int NV>
 __global__ __launch_bounds__(NT, 4) void gn_act_fwd_kernel(GnArgs a, char* __restrict__ out, float* __restrict__ stats,
                                                            unsigned long long* words, const double2* __restrict__ totals) {
   typedef typename Piece<T, VE>::reg reg_t;
   typedef typename Piece<T, VE>::mem mem_t;
-  __shared__ __attribute__((aligned(16))) float red[NT * (VE + 8)];
-  __shared__ __attribute__((aligned(16))) float chM[NT * VE];
-  float *const chW = red, *const chB = red + NT * VE;      // per channel mean, scale, offset: the last two once the sums are done
-  __shared__ float gs[MAX_GS], gmean[MAX_GS], grstd[MAX_GS];
+  // the threads' sums; afterwards, per channel, the mean and scale
+  __shared__ __attribute__((aligned(16))) float red[NT * VE < 2 * MAX_COL ? 2 * MAX_COL : NT * VE];
+  __shared__ __attribute__((aligned(16))) float chW[MAX_COL], chB[MAX_COL];      // per channel gamma * (1 + s), beta * (1 + s) + t
+  __shared__ float gsq[MAX_GS], gmean[MAX_GS], grstd[MAX_GS];
   __shared__ double2 tot[MAX_GS];
   __shared__ int missing;
   const Cut& q = a.cut;
-  drop_resolve(a.rng);
-  const int slab = blockIdx.x % q.nslab, rest = blockIdx.x / q.nslab;
-  const int me = rest % q.K, n = rest / q.K;
-  unsigned long long* const cluster = words + ((size_t)n * q.nslab + slab) * q.K * q.GS * 2;
-  const int GS = groups_of(a, slab);
-  const float Mf = (float)a.HW * (float)a.Cg;
+  const int rest = q.by_K.of(blockIdx.x), me = blockIdx.x - rest * q.K;      // a cluster's tiles start together
+  const int n = q.by_nslab.of(rest), slab = rest - n * q.nslab;
+  const Tile t = tile_of<VE>(a, slab, me, threadIdx.x);
 
+  const Affine<T> first = first_affine<T>(a, n, t);
+  // ---- the tile into registers ----
   reg_t x[NV];
-  Tile t;
-  bool again = false;
-  for (int k = me;;) {
-    // ---- the tile into registers, its groups' means and centred squares ----
-    t = tile_of<VE>(a, slab, k);
-    const int mine = t.active ? t.nrow - t.r0 : 0;
-    long long step;
-    const char* p = source<T, VE>(a, n, t, step);
-    int left = mine;      // (running pointers and counts: products with the sweep's number would all be kept across the loop)
+  {
+    Source<T, VE> src(a, n, t);
+    int left = t.mine;
+    forget(left);
     sweeps<NV>([&](auto i) __attribute__((always_inline)) {
-      x[i] = reg_t{};      // (so that no earlier tile's value stays alive behind the condition)
-      if (left > 0) x[i] = *(const mem_t*)p;
-      p += step;
+      x[i] = *(const mem_t*)src.p;
+      src.p += left > q.RPI ? src.step : 0;
       left -= q.RPI;
+      __builtin_amdgcn_sched_barrier(0);      // else all addresses are computed first and take the registers
     });
-    float s[VE];
+  }
+  each_channel<NT, T>(a, n, t, first, [&](int j, float2 wb) __attribute__((always_inline)) {
+    chW[j] = wb.x;
+    chB[j] = wb.y;
+  });
+  // ---- means and centred squares ----
+  float s[VE], m[VE];
 #pragma unroll
-    for (int e = 0; e < VE; ++e) s[e] = 0.f;
-    left = mine;
+  for (int e = 0; e < VE; ++e) s[e] = 0.f;
+  {
+    int left = t.mine;
+    forget(left);
     sweeps<NV>([&](auto i) __attribute__((always_inline)) {
       if (left > 0) {
         float f[VE];
@@ -296,101 +451,100 @@ __global__ __launch_bounds__(NT, 4) void gn_act_fwd_kernel(GnArgs a, char* __res
       }
       left -= q.RPI;
     });
-    reduce_groups<VE>(a, t, slab, s, red, gs);
-    const int kc = q.kcols == 1 ? 0 : k % q.kcols;
-    if (threadIdx.x < GS) gmean[threadIdx.x] = gs[threadIdx.x] / fmaxf((float)t.nrow * (float)columns_of(a, slab, kc, threadIdx.x, VE), 1.f);
-    __syncthreads();
-    for (int j = threadIdx.x; j < t.ce - t.cb; j += NT) chM[j] = gmean[(t.cb + j) / a.Cg - slab * q.GS];
-    __syncthreads();
-    float m[VE];
-    read_channels<VE>(chM, t.piece, m);
+    tile_means<VE>(a, t, slab, s, m, red, gmean);
 #pragma unroll
     for (int e = 0; e < VE; ++e) s[e] = 0.f;
-    left = mine;
+    left = t.mine;
+    forget(left);
     sweeps<NV>([&](auto i) __attribute__((always_inline)) {
       if (left > 0) {
         float f[VE];
         forget(x[i]);
         unpack<T, VE>(x[i], f);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) { const float d = f[e] - m[e]; s[e] += d * d; }
+        for (int e = 0; e < VE; ++e) { const float d = f[e] - m[e]; s[e] = __builtin_fmaf(d, d, s[e]); }
       }
       left -= q.RPI;
     });
-    reduce_groups<VE>(a, t, slab, s, red, gs);
-    if (q.K == 1 || q.phase == PH_RESULT) break;
-    if (threadIdx.x < GS) {
-      publish(cluster + ((size_t)k * q.GS + threadIdx.x) * 2, gmean[threadIdx.x]);
-      publish(cluster + ((size_t)k * q.GS + threadIdx.x) * 2 + 1, gs[threadIdx.x]);
-    }
-    if (q.phase == PH_SUMS) return;
-    if (again) break;
-    const int miss = gather<VE, true>(a, slab, cluster, &missing, tot);
-    if (miss >= 0) k = miss;
-    else if (k == me) break;
-    else { k = me; again = true; }
+    group_sums<VE>(a, t, slab, s, red, gsq);
   }
-  __syncthreads();
+  const int GS = groups_of(a, slab), g = threadIdx.x;
   if (q.K == 1) {
-    if (threadIdx.x < GS) grstd[threadIdx.x] = 1.0f / sqrtf(gs[threadIdx.x] / Mf + a.eps);
+    if (g < GS) grstd[g] = 1.0f / sqrtf(gsq[g] / ((float)a.HW * (float)a.Cg) + a.eps);
   } else {
-    if (threadIdx.x < GS) {
-      if (q.phase == PH_RESULT) tot[threadIdx.x] = totals[((size_t)n * q.nslab + slab) * q.GS + threadIdx.x];
-      const double M = (double)a.HW * (double)a.Cg, mean = tot[threadIdx.x].x / M;
-      const double var = fmax(tot[threadIdx.x].y / M - mean * mean, 0.0);
-      gmean[threadIdx.x] = (float)mean;
+    if (q.phase != PH_RESULT) {
+      unsigned long long* const cluster = words + ((size_t)n * q.nslab + slab) * q.K * q.GS * 2;
+      for (int k = me;;) {
+        if (g < GS) {
+          publish(cluster + ((size_t)k * q.GS + g) * 2, gmean[g]);
+          publish(cluster + ((size_t)k * q.GS + g) * 2 + 1, gsq[g]);
+        }
+        if (q.phase == PH_SUMS) return;
+        k = gather<VE, true>(a, slab, cluster, &missing, tot);
+        if (k < 0) break;
+        help_forward<T, VE>(a, n, slab, k, red, gmean, gsq);
+      }
+    }
+    if (g < GS) {
+      const double2 sum = q.phase == PH_RESULT ? totals[((size_t)n * q.nslab + slab) * q.GS + g] : tot[g];
+      const double M = (double)a.HW * (double)a.Cg, mean = sum.x / M;
+      const double var = fmax(sum.y / M - mean * mean, 0.0);
+      gmean[g] = (float)mean;
       // a NaN sum stays one: fmax would drop it
-      grstd[threadIdx.x] = tot[threadIdx.x].y == tot[threadIdx.x].y ? (float)(1.0 / sqrt(var + (double)a.eps)) : __builtin_nanf("");
+      grstd[g] = sum.y == sum.y ? (float)(1.0 / sqrt(var + (double)a.eps)) : __builtin_nanf("");
     }
   }
   __syncthreads();
-  if (me == 0 && threadIdx.x < GS) {
-    const size_t i = ((size_t)n * a.G + slab * q.GS + threadIdx.x) * 2;
-    stats[i] = gmean[threadIdx.x];
-    stats[i + 1] = grstd[threadIdx.x];
+  if (me == 0 && g < GS) {
+    const size_t i = ((size_t)n * a.G + slab * q.GS + g) * 2;
+    stats[i] = gmean[g];
+    stats[i + 1] = grstd[g];
   }
-  for (int j = threadIdx.x; j < t.ce - t.cb; j += NT) {
-    const int g = (t.cb + j) / a.Cg - slab * q.GS;
-    const float2 wb = affine<T>(a, n, t.cb + j);
-    chM[j] = gmean[g];
-    chW[j] = wb.x * grstd[g];
-    chB[j] = wb.y;
+  float *const chM = red, *const chS = red + MAX_COL;
+  for (int j = g; j < t.ce - t.cb; j += NT) {
+    const int gj = q.by_Cg.of(t.cb + j) - slab * q.GS;
+    chM[j] = gmean[gj];
+    chS[j] = chW[j] * grstd[gj];
   }
   __syncthreads();
-  if (!t.active) return;
-  float m[VE], sc[VE], bb[VE];
+  if (t.mine <= 0) return;
+  // ---- the result ----
+  float sc[VE], bb[VE];
   read_channels<VE>(chM, t.piece, m);
-  read_channels<VE>(chW, t.piece, sc);
+  read_channels<VE>(chS, t.piece, sc);
   read_channels<VE>(chB, t.piece, bb);
+  if (a.drop) drop_resolve(a.rng);
   long long o = ((long long)n * a.HW + t.row0 + t.r0) * a.C + t.c;
   const long long ostep = (long long)q.RPI * a.C;
-  int left = t.nrow - t.r0;
+  int left = t.mine;
+  forget(left);
   sweeps<NV>([&](auto i) __attribute__((always_inline)) {
     if (left > 0) {
       float f[VE];
       forget(x[i]);
       unpack<T, VE>(x[i], f);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) f[e] = (f[e] - m[e]) * sc[e] + bb[e];
+      for (int e = 0; e < VE; ++e) f[e] = __builtin_fmaf(f[e] - m[e], sc[e], bb[e]);
       if (a.act) {
 #pragma unroll
         for (int e = 0; e < VE; ++e) f[e] = silu_f(f[e]);
       }
       if (a.drop) drop_apply<VE>(a.rng, (unsigned long long)o, f);
-      *(mem_t*)(out + o * (long long)sizeof(T)) = pack<T, VE>(f);
+      __builtin_nontemporal_store(pack<T, VE>(f), (mem_t*)(out + o * (long long)sizeof(T)));
     }
     o += ostep;
     left -= q.RPI;
   });
 }
 
+// ---- backward ----
 // dscale, dshift of one (n, c) and its share of dgamma, dbeta
 template <typename T>
 __device__ __forceinline__ void channel_done(const GnArgs& a, int n, int c, float A, float B, float2* ab, char* dfilm) {
   float gain = 1.0f;
   if (a.film_kind) {
     gain += film_at<T>(a, (long long)n * a.film_ld + c);
-    const float ds = a.gamma[c] * B + a.beta[c] * A;
+    const float ds = __builtin_fmaf(a.gamma[c], B, a.beta[c] * A);
     const long long i = (long long)n * 2 * a.C + c;
     if (a.film_kind == 1) { ((float*)dfilm)[i] = ds; ((float*)dfilm)[i + a.C] = A; }
     else { ((T*)dfilm)[i] = (T)ds; ((T*)dfilm)[i + a.C] = (T)A; }
@@ -398,7 +552,125 @@ __device__ __forceinline__ void channel_done(const GnArgs& a, int n, int c, floa
   ab[(long long)n * a.C + c] = make_float2(gain * A, gain * B);
 }
 
-template <typename T, int VE, int NV>
+// d: dy -> gv, f: x -> xc, of one piece; o = its index in dy
+template <int VE>
+__device__ __forceinline__ void gradient_of(const GnArgs& a, long long o, const float* m, const float* sc, const float* bb, float* f, float* d) {
+  if (a.drop) drop_apply<VE>(a.rng, (unsigned long long)o, d);
+#pragma unroll
+  for (int e = 0; e < VE; ++e) f[e] -= m[e];
+  if (a.act) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const float v = __builtin_fmaf(f[e], sc[e], bb[e]);
+      const float sg = __builtin_amdgcn_rcpf(1.0f + __expf(-v));
+      d[e] *= sg * __builtin_fmaf(v, 1.0f - sg, 1.0f);
+    }
+  }
+}
+
+struct BwdShared {
+  float *redA, *redB, *chM, *chW, *chA, *chB, *gmean, *grstd, *gm1, *gm2;
+};
+// per channel mean, gamma * (1 + s), offset, scale into LDS
+template <int NT, typename T>
+__device__ __forceinline__ void bwd_channels(const GnArgs& a, int n, int slab, const Tile& t, const Affine<T>& first, const BwdShared& h) {
+  each_channel<NT, T>(a, n, t, first, [&](int j, float2 wb) __attribute__((always_inline)) {
+    const int gj = a.cut.by_Cg.of(t.cb + j) - slab * a.cut.GS;
+    h.chM[j] = h.gmean[gj];
+    h.chW[j] = wb.x;
+    h.chA[j] = wb.y;
+    h.chB[j] = wb.x * h.grstd[gj];
+  });
+  __syncthreads();
+}
+// The threads' channel sums A, B (of gv and gv * xc) -> those of the tile (chA, chB; done(j, A, B) for each) and of its groups (gm1, gm2:
+// sums of g and g * xhat).
+template <int NT, int VE, typename F>
+__device__ __forceinline__ void join_gradients(const GnArgs& a, const Tile& t, int slab, const float* A, const float* B, const BwdShared& h, F done) {
+  const Cut& q = a.cut;
+  const int thread = fresh_thread();
+  const int RS = q.PP * VE + 8, ncol = t.ce - t.cb;
+  if (t.r0 < q.RPI) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      h.redA[t.r0 * RS + t.piece * VE + e] = A[e];
+      h.redB[t.r0 * RS + t.piece * VE + e] = B[e];
+    }
+  }
+  __syncthreads();
+  const int rows = min(q.RPI, t.nrow);
+  const int parts = ncol < NT ? NT / ncol : 1;
+  int nr = rows, rs = RS;
+  if (parts > 1) {
+    const int p = thread / ncol, j = thread - p * ncol;
+    float sa = 0.f, sb = 0.f;
+    if (p < parts) {
+#pragma unroll 4
+      for (int r = p; r < rows; r += parts) { sa += h.redA[r * RS + j]; sb += h.redB[r * RS + j]; }
+    }
+    __syncthreads();
+    if (p < parts) { h.redA[p * ncol + j] = sa; h.redB[p * ncol + j] = sb; }
+    __syncthreads();
+    nr = min(parts, rows);
+    rs = ncol;
+  }
+  for (int j = thread; j < ncol; j += NT) {
+    float sa = 0.f, sb = 0.f;
+    for (int r = 0; r < nr; ++r) { sa += h.redA[r * rs + j]; sb += h.redB[r * rs + j]; }
+    sb *= h.grstd[q.by_Cg.of(t.cb + j) - slab * q.GS];
+    h.chA[j] = sa;
+    h.chB[j] = sb;
+    done(j, sa, sb);
+  }
+  __syncthreads();
+  const int g = thread >> q.logW, W = 1 << q.logW, l = thread & (W - 1);
+  const int c0 = slab * q.S + g * a.Cg;
+  float s1 = 0.f, s2 = 0.f;
+  if (g < groups_of(a, slab)) {
+    for (int j = max(c0, t.cb) - t.cb + l; j < min(c0 + a.Cg, t.ce) - t.cb; j += W) {
+      s1 += h.chA[j] * h.chW[j];
+      s2 += h.chB[j] * h.chW[j];
+    }
+  }
+  for (int o = W >> 1; o > 0; o >>= 1) {
+    s1 += __shfl_xor(s1, o);
+    s2 += __shfl_xor(s2, o);
+  }
+  if (l == 0 && g < q.GS) {
+    h.gm1[g] = s1;
+    h.gm2[g] = s2;
+  }
+  __syncthreads();
+}
+
+template <int NT, typename T, int VE>
+__device__ __forceinline__ void help_backward(const GnArgs& a, int n, int slab, int k, const char* dy, const BwdShared& h) {
+  typedef typename Piece<T, VE>::mem mem_t;
+  const Tile t = tile_of<VE>(a, slab, k, fresh_thread());
+  bwd_channels<NT, T>(a, n, slab, t, first_affine<T>(a, n, t), h);
+  float m[VE], sc[VE], bb[VE], A[VE], B[VE];
+  read_channels<VE>(h.chM, t.piece, m);
+  read_channels<VE>(h.chA, t.piece, bb);
+  read_channels<VE>(h.chB, t.piece, sc);
+#pragma unroll
+  for (int e = 0; e < VE; ++e) A[e] = B[e] = 0.f;
+  Source<T, VE> src(a, n, t);
+  long long o = ((long long)n * a.HW + t.row0 + t.r0) * a.C + t.c;
+#pragma unroll 1
+  for (int left = t.mine; left > 0; left -= a.cut.RPI) {
+    float f[VE], d[VE];
+    unpack<T, VE>(*(const mem_t*)src.p, f);
+    unpack<T, VE>(*(const mem_t*)(dy + o * (long long)sizeof(T)), d);
+    gradient_of<VE>(a, o, m, sc, bb, f, d);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) { A[e] += d[e]; B[e] = __builtin_fmaf(d[e], f[e], B[e]); }
+    src.p += src.step;
+    o += (long long)a.cut.RPI * a.C;
+  }
+  join_gradients<NT, VE>(a, t, slab, A, B, h, [](int, float, float) {});
+}
+
+template <int NT, typename T, int VE, int NV>
 __global__ __launch_bounds__(NT, 2) void gn_act_bwd_kernel(GnArgs a, const float* __restrict__ stats, const char* __restrict__ dy,
                                                            char* __restrict__ d0, char* __restrict__ d1, unsigned long long* words,
                                                            const double2* __restrict__ totals, float2* __restrict__ part,
@@ -406,182 +678,126 @@ __global__ __launch_bounds__(NT, 2) void gn_act_bwd_kernel(GnArgs a, const float
   typedef typename Piece<T, VE>::reg reg_t;
   typedef typename Piece<T, VE>::mem mem_t;
   __shared__ __attribute__((aligned(16))) float redA[NT * (VE + 8)], redB[NT * (VE + 8)];
-  // per channel: mean, gamma * (1 + s), the offset (then A), B
-  __shared__ __attribute__((aligned(16))) float chM[NT * VE], chW[NT * VE], chA[NT * VE], chB[NT * VE];
+  // per channel: mean, gamma * (1 + s), the offset (then A), the scale (then B)
+  __shared__ __attribute__((aligned(16))) float chM[MAX_COL], chW[MAX_COL], chA[MAX_COL], chB[MAX_COL];
   __shared__ float gmean[MAX_GS], grstd[MAX_GS], gm1[MAX_GS], gm2[MAX_GS];
   __shared__ double2 tot[MAX_GS];
   __shared__ int missing;
+  BwdShared h;      // (assigned: an initialiser list would be a constant with LDS addresses)
+  h.redA = redA; h.redB = redB; h.chM = chM; h.chW = chW; h.chA = chA; h.chB = chB;
+  h.gmean = gmean; h.grstd = grstd; h.gm1 = gm1; h.gm2 = gm2;
   const Cut& q = a.cut;
-  drop_resolve(a.rng);
-  const int slab = blockIdx.x % q.nslab, rest = blockIdx.x / q.nslab;
-  const int me = rest % q.K, n = rest / q.K;
-  unsigned long long* const cluster = words + ((size_t)n * q.nslab + slab) * q.K * q.GS * 2;
-  const int GS = groups_of(a, slab);
-  const float Mf = (float)a.HW * (float)a.Cg;
-  if (threadIdx.x < GS) {
-    const size_t i = ((size_t)n * a.G + slab * q.GS + threadIdx.x) * 2;
-    gmean[threadIdx.x] = stats[i];
-    grstd[threadIdx.x] = stats[i + 1];
-  }
-  __syncthreads();
+  const int rest = q.by_K.of(blockIdx.x), me = blockIdx.x - rest * q.K;      // a cluster's tiles start together
+  const int n = q.by_nslab.of(rest), slab = rest - n * q.nslab;
+  const Tile t = tile_of<VE>(a, slab, me, threadIdx.x);
+  const int GS = groups_of(a, slab), g = threadIdx.x;
+  const long long o0 = ((long long)n * a.HW + t.row0 + t.r0) * a.C + t.c, ostep = (long long)q.RPI * a.C;
 
   reg_t x[NV];
   float gv[NV][VE];
-  Tile t;
-  bool again = false;
-  for (int k = me;;) {
-    t = tile_of<VE>(a, slab, k);
-    const int mine = t.active ? t.nrow - t.r0 : 0;
-    const long long o0 = ((long long)n * a.HW + t.row0 + t.r0) * a.C + t.c, ostep = (long long)q.RPI * a.C;
-    long long step;
-    const char* p = source<T, VE>(a, n, t, step);
-    reg_t g[NV];
-    int left = mine;
-    const char* pd = dy + o0 * (long long)sizeof(T);
+  {
+    // ---- the tile into registers ----
+    const Affine<T> first = first_affine<T>(a, n, t);
+    const float2 stat = ((const float2*)stats)[(size_t)n * a.G + slab * q.GS + min(g, GS - 1)];
+    reg_t dd[NV];
+    Source<T, VE> src(a, n, t);
+    const char* pd = dy + (t.mine > 0 ? o0 : ((long long)n * a.HW + t.row0) * a.C + t.cb) * (long long)sizeof(T);
+    int left = t.mine;
+    forget(left);
     sweeps<NV>([&](auto i) __attribute__((always_inline)) {
-      x[i] = g[i] = reg_t{};      // (so that no earlier tile's value stays alive behind the condition)
-      if (left > 0) {
-        x[i] = *(const mem_t*)p;
-        g[i] = *(const mem_t*)pd;
-      }
-      p += step;
-      pd += ostep * (long long)sizeof(T);
+      x[i] = *(const mem_t*)src.p;
+      dd[i] = *(const mem_t*)pd;
+      src.p += left > q.RPI ? src.step : 0;
+      pd += left > q.RPI ? ostep * (long long)sizeof(T) : 0;
       left -= q.RPI;
+      __builtin_amdgcn_sched_barrier(0);      // else all addresses are computed first and take the registers
     });
-    for (int j = threadIdx.x; j < t.ce - t.cb; j += NT) {
-      const int gj = (t.cb + j) / a.Cg - slab * q.GS;
-      const float2 wb = affine<T>(a, n, t.cb + j);
-      chM[j] = gmean[gj];
-      chW[j] = wb.x;
-      chA[j] = wb.y;
-      chB[j] = wb.x * grstd[gj];
+    if (g < GS) {
+      gmean[g] = stat.x;
+      grstd[g] = stat.y;
     }
+    if (a.drop) drop_resolve(a.rng);
     __syncthreads();
+    bwd_channels<NT, T>(a, n, slab, t, first, h);
+    // ---- gv and the channels' sums ----
     float m[VE], bb[VE], sc[VE], A[VE], B[VE];
     read_channels<VE>(chM, t.piece, m);
     read_channels<VE>(chA, t.piece, bb);
     read_channels<VE>(chB, t.piece, sc);
 #pragma unroll
     for (int e = 0; e < VE; ++e) A[e] = B[e] = 0.f;
-    left = mine;
+    left = t.mine;
+    forget(left);
     long long o = o0;
     sweeps<NV>([&](auto i) __attribute__((always_inline)) {
       if (left > 0) {
         float f[VE], d[VE];
         forget(x[i]);
         unpack<T, VE>(x[i], f);
-        unpack<T, VE>(g[i], d);
-        if (a.drop) drop_apply<VE>(a.rng, (unsigned long long)o, d);
-#pragma unroll
-        for (int e = 0; e < VE; ++e) f[e] -= m[e];
-        if (a.act) {
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            const float v = f[e] * sc[e] + bb[e];
-            const float sg = __builtin_amdgcn_rcpf(1.0f + __expf(-v));
-            d[e] *= sg * (1.0f + v * (1.0f - sg));
-          }
-        }
+        unpack<T, VE>(dd[i], d);
+        gradient_of<VE>(a, o, m, sc, bb, f, d);
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           gv[i][e] = d[e];
           A[e] += d[e];
-          B[e] += d[e] * f[e];
+          B[e] = __builtin_fmaf(d[e], f[e], B[e]);
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < VE; ++e) gv[i][e] = 0.f;
       }
       o += ostep;
       left -= q.RPI;
     });
-    // ---- channel sums over the tile's pixels ----
-    const int RS = q.PP * VE + 8, ncol = t.ce - t.cb;
-    if (t.r0 < q.RPI) {
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        redA[t.r0 * RS + t.piece * VE + e] = A[e];
-        redB[t.r0 * RS + t.piece * VE + e] = B[e];
-      }
-    }
-    __syncthreads();
-    const int parts = ncol < NT ? NT / ncol : 1;
-    if (parts > 1) {
-      const int h = threadIdx.x / ncol, j = threadIdx.x - h * ncol;
-      float sa = 0.f, sb = 0.f;
-      if (h < parts) {
-        for (int r = h; r < q.RPI; r += parts) { sa += redA[r * RS + j]; sb += redB[r * RS + j]; }
-      }
-      __syncthreads();
-      if (h < parts) { redA[h * ncol + j] = sa; redB[h * ncol + j] = sb; }
-      __syncthreads();
-    }
-    const int nr = parts > 1 ? min(parts, q.RPI) : q.RPI, rs = parts > 1 ? ncol : RS;
-    const int kr = q.kcols == 1 ? k : k / q.kcols;
-    for (int j = threadIdx.x; j < ncol; j += NT) {
-      float sa = 0.f, sb = 0.f;
-      for (int r = 0; r < nr; ++r) { sa += redA[r * rs + j]; sb += redB[r * rs + j]; }
-      sb *= grstd[(t.cb + j) / a.Cg - slab * q.GS];
-      chA[j] = sa;
-      chB[j] = sb;
-      if (q.krows > 1) part[((size_t)n * q.krows + kr) * a.C + t.cb + j] = make_float2(sa, sb);
+    join_gradients<NT, VE>(a, t, slab, A, B, h, [&](int j, float sa, float sb) __attribute__((always_inline)) {
+      if (q.krows > 1) part[((size_t)n * q.krows + (q.kcols > 1 ? me / q.kcols : me)) * a.C + t.cb + j] = make_float2(sa, sb);
       else channel_done<T>(a, n, t.cb + j, sa, sb, ab, dfilm);
-    }
-    __syncthreads();
-    // ---- the groups' sums of g and g * xhat ----
-    {
-      const int g2 = threadIdx.x / q.W, l = threadIdx.x - g2 * q.W;
-      const int c0 = slab * q.S + g2 * a.Cg;
-      float s1 = 0.f, s2 = 0.f;
-      if (g2 < GS) {
-        for (int j = max(c0, t.cb) - t.cb + l; j < min(c0 + a.Cg, t.ce) - t.cb; j += q.W) {
-          s1 += mul_rounded(chA[j], chW[j]);
-          s2 += mul_rounded(chB[j], chW[j]);
-        }
-      }
-      for (int o = q.W >> 1; o > 0; o >>= 1) {
-        s1 += __shfl_xor(s1, o);
-        s2 += __shfl_xor(s2, o);
-      }
-      if (l == 0 && g2 < GS) {
-        gm1[g2] = s1 / Mf;
-        gm2[g2] = s2 / Mf;
-        if (q.K > 1 && q.phase != PH_RESULT) {
-          publish(cluster + ((size_t)k * q.GS + g2) * 2, s1);
-          publish(cluster + ((size_t)k * q.GS + g2) * 2 + 1, s2);
-        }
-      }
-    }
-    if (q.phase == PH_SUMS) return;
-    if (q.K == 1 || q.phase == PH_RESULT || again) break;
-    const int miss = gather<VE, false>(a, slab, cluster, &missing, tot);
-    if (miss >= 0) k = miss;
-    else if (k == me) break;
-    else { k = me; again = true; }
+    });
   }
-  __syncthreads();
+  const float Mf = (float)a.HW * (float)a.Cg;
   if (q.K > 1) {
-    if (threadIdx.x < GS) {
-      if (q.phase == PH_RESULT) tot[threadIdx.x] = totals[((size_t)n * q.nslab + slab) * q.GS + threadIdx.x];
-      const double M = (double)a.HW * (double)a.Cg;
-      gm1[threadIdx.x] = (float)(tot[threadIdx.x].x / M);
-      gm2[threadIdx.x] = (float)(tot[threadIdx.x].y / M);
+    bool helped = false;
+    if (q.phase != PH_RESULT) {
+      unsigned long long* const cluster = words + ((size_t)n * q.nslab + slab) * q.K * q.GS * 2;
+      for (int k = me;;) {
+        if (g < GS) {
+          publish(cluster + ((size_t)k * q.GS + g) * 2, gm1[g]);
+          publish(cluster + ((size_t)k * q.GS + g) * 2 + 1, gm2[g]);
+        }
+        if (q.phase == PH_SUMS) return;
+        k = gather<VE, false>(a, slab, cluster, &missing, tot);
+        if (k < 0) break;
+        help_backward<NT, T, VE>(a, n, slab, k, dy, h);
+        helped = true;
+      }
     }
-    __syncthreads();
-  }
-  for (int j = threadIdx.x; j < t.ce - t.cb; j += NT) {
-    const int g = (t.cb + j) / a.Cg - slab * q.GS;
-    chA[j] = gm1[g];
-    chB[j] = gm2[g] * grstd[g];
-    redA[j] = grstd[g];
+    if (g < GS) {
+      const double2 sum = q.phase == PH_RESULT ? totals[((size_t)n * q.nslab + slab) * q.GS + g] : tot[g];
+      const double M = (double)a.HW * (double)a.Cg;
+      gm1[g] = (float)(sum.x / M);
+      gm2[g] = (float)(sum.y / M);
+    }
+    if (helped && q.kcols > 1) {      // another column chunk's channels are in LDS now
+      __syncthreads();
+      bwd_channels<NT, T>(a, n, slab, t, first_affine<T>(a, n, t), h);
+    }
+  } else if (g < GS) {
+    gm1[g] /= Mf;
+    gm2[g] /= Mf;
   }
   __syncthreads();
-  if (!t.active) return;
+  for (int j = threadIdx.x; j < t.ce - t.cb; j += NT) {
+    const int gj = q.by_Cg.of(t.cb + j) - slab * q.GS;
+    chA[j] = gm1[gj];
+    chB[j] = gm2[gj] * grstd[gj];
+    redA[j] = grstd[gj];
+  }
+  __syncthreads();
+  if (t.mine <= 0) return;
+  // ---- the result ----
   const bool second = t.c >= a.C0;
   const long long ld = second ? a.C - a.C0 : a.C0;
   char* o = (second ? d1 : d0) + (((long long)n * a.HW + t.row0 + t.r0) * ld + (t.c - (second ? a.C0 : 0))) * (long long)sizeof(T);
-  const long long ostep = ld * q.RPI * (long long)sizeof(T);
-  int left = t.nrow - t.r0;
+  const long long ostep2 = ld * (q.RPI * (int)sizeof(T));
+  int left = t.mine;
+  forget(left);
   float m[VE], gw[VE], m1[VE], m2[VE], rs[VE];
   read_channels<VE>(chM, t.piece, m);
   read_channels<VE>(chW, t.piece, gw);
@@ -593,17 +809,18 @@ __global__ __launch_bounds__(NT, 2) void gn_act_bwd_kernel(GnArgs a, const float
       float f[VE];
       forget(x[i]);
       unpack<T, VE>(x[i], f);
+      // (g is rounded before sum(g) / M is taken off: with one value a group they cancel exactly)
 #pragma unroll
-      for (int e = 0; e < VE; ++e) f[e] = rs[e] * ((mul_rounded(gv[i][e], gw[e]) - m1[e]) - (f[e] - m[e]) * m2[e]);
-      *(mem_t*)o = pack<T, VE>(f);
+      for (int e = 0; e < VE; ++e) f[e] = rs[e] * __builtin_fmaf(m[e] - f[e], m2[e], gv[i][e] * gw[e] - m1[e]);
+      __builtin_nontemporal_store(pack<T, VE>(f), (mem_t*)o);
     }
-    o += ostep;
+    o += ostep2;
     left -= q.RPI;
   });
 }
 
 // the words of one cluster added up, between PH_SUMS and PH_RESULT: one workgroup per (sample, slab)
-template <int VE, bool MOMENTS>
+template <int NT, int VE, bool MOMENTS>
 __global__ __launch_bounds__(NT) void gn_act_total_kernel(GnArgs a, const unsigned long long* words, double2* __restrict__ totals) {
   __shared__ double2 tot[MAX_GS];
   __shared__ int missing;
@@ -614,20 +831,20 @@ __global__ __launch_bounds__(NT) void gn_act_total_kernel(GnArgs a, const unsign
 }
 
 // zeroes the clusters' words (a kernel, so that it may be captured)
-__global__ __launch_bounds__(NT) void gn_act_clear_kernel(ulonglong2* words, long long n) {
-  const long long i = (long long)blockIdx.x * NT + threadIdx.x;
+__global__ __launch_bounds__(NT_AUX) void gn_act_clear_kernel(ulonglong2* words, long long n) {
+  const long long i = (long long)blockIdx.x * NT_AUX + threadIdx.x;
   if (i < n) words[i] = make_ulonglong2(0, 0);
 }
 
 // part [N][krows][C] -> ab [N][C], dfilm: 64 channels a workgroup, four threads a channel
 template <typename T>
-__global__ __launch_bounds__(NT) void gn_act_film_kernel(GnArgs a, const float2* __restrict__ part, float2* __restrict__ ab, char* __restrict__ dfilm) {
-  __shared__ float2 red[NT];
+__global__ __launch_bounds__(NT_AUX) void gn_act_film_kernel(GnArgs a, const float2* __restrict__ part, float2* __restrict__ ab, char* __restrict__ dfilm) {
+  __shared__ float2 red[NT_AUX];
   const int cblk = (a.C + 63) / 64;
   const int n = blockIdx.x / cblk, c = (blockIdx.x - n * cblk) * 64 + (threadIdx.x & 63), h = threadIdx.x >> 6;
   float A = 0.f, B = 0.f;
   if (c < a.C) {
-    for (int k = h; k < a.cut.krows; k += NT / 64) {
+    for (int k = h; k < a.cut.krows; k += NT_AUX / 64) {
       const float2 v = part[((size_t)n * a.cut.krows + k) * a.C + c];
       A += v.x;
       B += v.y;
@@ -637,14 +854,14 @@ __global__ __launch_bounds__(NT) void gn_act_film_kernel(GnArgs a, const float2*
   __syncthreads();
   if (h == 0 && c < a.C) {
 #pragma unroll
-    for (int j = 1; j < NT / 64; ++j) { A += red[threadIdx.x + 64 * j].x; B += red[threadIdx.x + 64 * j].y; }
+    for (int j = 1; j < NT_AUX / 64; ++j) { A += red[threadIdx.x + 64 * j].x; B += red[threadIdx.x + 64 * j].y; }
     channel_done<T>(a, n, c, A, B, ab, dfilm);
   }
 }
 
 // ab [N][C] -> dgamma, dbeta: 16 channels a workgroup, 16 threads a channel
-__global__ __launch_bounds__(NT) void gn_act_param_kernel(const float2* __restrict__ ab, int N, int C, float* __restrict__ dgamma, float* __restrict__ dbeta) {
-  __shared__ float2 red[NT];
+__global__ __launch_bounds__(NT_AUX) void gn_act_param_kernel(const float2* __restrict__ ab, int N, int C, float* __restrict__ dgamma, float* __restrict__ dbeta) {
+  __shared__ float2 red[NT_AUX];
   const int c = blockIdx.x * 16 + (threadIdx.x & 15), h = threadIdx.x >> 4;
   float A = 0.f, B = 0.f;
   if (c < C) {
@@ -664,13 +881,25 @@ __global__ __launch_bounds__(NT) void gn_act_param_kernel(const float2* __restri
   }
 }
 
+Div div_by(int d) {
+  int l = 0;
+  while ((1ll << l) < d) ++l;
+  return Div{(uint32_t)d, (uint32_t)(((1ull << (24 + l)) + d - 1) / d), (uint32_t)(24 + l)};
+}
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
-// register-resident sweeps per type of piece
-constexpr int NV_FWD = 16, NV_BWD = 12, NV_NARROW = 32;
-int max_sweeps(int ve, bool backward) { return ve <= 2 ? NV_NARROW : (backward ? NV_BWD : NV_FWD); }
+// Sweeps that a tile may have (instantiations): 16-byte pieces take the smallest count that holds a sample's pixels, else the largest.
+constexpr int SWEEPS_FWD[] = {2, 4, 8, 16}, SWEEPS_BWD[] = {2, 4, 8, 12}, SWEEPS_NARROW = 16;
+int sweeps_for(int ve, int esz, bool backward, long long needed) {
+  if (ve * esz < 16) return SWEEPS_NARROW;
+  const int* list = backward ? SWEEPS_BWD : SWEEPS_FWD;
+  int i = 0;
+  while (i < 3 && list[i] < needed) ++i;
+  return list[i];
+}
 
 int cut_up(const ivid_gn_act_desc* d, bool backward, GnArgs* a, int* ve_out) {
+  const int NT = backward ? NT_BWD : NT_FWD;
   const int esz = ivid_esz(d->dtype);
   // the widest piece that every row of every tensor is a whole number of
   int ve = 16 / esz;
@@ -680,13 +909,14 @@ int cut_up(const ivid_gn_act_desc* d, bool backward, GnArgs* a, int* ve_out) {
            !((uintptr_t)d->src1 % (v * esz));
   };
   while (ve > 1 && !fits(ve)) ve >>= 1;
+  const int wide = NT < MAX_COL / ve ? NT : MAX_COL / ve;      // pieces of a tile's row at most
   const int C = a->C, Cg = a->Cg;
   const long long unit = (long long)Cg / gcd(Cg, ve) * ve;     // whole groups and whole pieces
   Cut& q = a->cut;
   long long S = unit;
-  while (S < C && S * esz < 128 && (S + unit) / Cg <= MAX_GS && (S + unit) / ve <= NT) S += unit;
+  while (S < C && S * esz < 128 && (S + unit) / Cg <= MAX_GS && (S + unit) / ve <= wide) S += unit;
   // whole 128-byte lines, if a few more groups make them
-  for (long long s = S; s <= 4 * S && s <= C && s / Cg <= MAX_GS && s / ve <= NT; s += unit)
+  for (long long s = S; s <= 4 * S && s <= C && s / Cg <= MAX_GS && s / ve <= wide; s += unit)
     if (s * esz % 128 == 0) { S = s; break; }
   if (S > C) S = C;            // C is a multiple of the unit
   q.S = (int)S;
@@ -694,14 +924,13 @@ int cut_up(const ivid_gn_act_desc* d, bool backward, GnArgs* a, int* ve_out) {
   q.GS = (int)(S / Cg);
   if (q.GS > MAX_GS) return ivid_set_error("gn_act: internal: too many groups in a slab", hipSuccess);
   const int pieces = (int)(S / ve);
-  q.kcols = (pieces + NT - 1) / NT;
+  q.kcols = (pieces + wide - 1) / wide;
   q.PP = (pieces + q.kcols - 1) / q.kcols;
   q.RPI = NT / q.PP;
-  q.W = 64;
-  while (q.W * q.GS > NT) q.W >>= 1;
-  const int most = max_sweeps(ve, backward);
-  q.nv = (int)(((long long)d->HW + q.RPI - 1) / q.RPI);
-  if (q.nv > most) q.nv = most;
+  for (q.seg = 1, q.logseg = 0; q.seg < ve && Cg % (2 * q.seg) == 0;) { q.seg *= 2; ++q.logseg; }
+  q.logW = 6;
+  while ((q.GS << q.logW) > NT) --q.logW;
+  q.nv = sweeps_for(ve, esz, backward, ((long long)d->HW + q.RPI - 1) / q.RPI);
   q.rows = q.RPI * q.nv;
   q.krows = (int)(((long long)d->HW + q.rows - 1) / q.rows);
   q.polls = d->max_polls > 0 ? d->max_polls : MAX_POLLS;
@@ -710,6 +939,11 @@ int cut_up(const ivid_gn_act_desc* d, bool backward, GnArgs* a, int* ve_out) {
   q.K = tiles < (1 << 24) ? q.krows * q.kcols : 0;
   if (!q.K || (long long)d->N * ((C + 63) / 64) >= (1 << 24))
     return ivid_set_error("gn_act: too many tiles for one launch", hipSuccess);
+  q.by_nslab = div_by(q.nslab);
+  q.by_K = div_by(q.K);
+  q.by_PP = div_by(q.PP);
+  q.by_Cg = div_by(Cg);
+  q.by_runs = div_by(Cg >> q.logseg);
   return 0;
 }
 
@@ -753,14 +987,14 @@ Scratch layout(const ivid_gn_act_desc* d, const GnArgs& a, bool backward) {
 
 int clear_words(const Scratch& s, void* scratch, hipStream_t stream) {
   if (!s.words || s.totals) return 0;      // two launches: every word is written before any is read
-  const long long n = s.words / 16, blocks = (n + NT - 1) / NT;
+  const long long n = s.words / 16, blocks = (n + NT_AUX - 1) / NT_AUX;
   if (blocks >= (1 << 24)) return ivid_set_error("gn_act: too many tiles for one launch", hipSuccess);
-  hipLaunchKernelGGL(gn_act_clear_kernel, dim3((unsigned)blocks), dim3(NT), 0, stream, (ulonglong2*)scratch, n);
+  hipLaunchKernelGGL(gn_act_clear_kernel, dim3((unsigned)blocks), dim3(NT_AUX), 0, stream, (ulonglong2*)scratch, n);
   return 0;
 }
 
 // `run` launches the kernel once, or as sums - totals - results
-template <bool MOMENTS, typename Run>
+template <int NT, bool MOMENTS, typename Run>
 void run_phases(GnArgs& a, const ivid_gn_act_desc* d, int ve, const Scratch& s, void* scratch, hipStream_t st, Run run) {
   if (!s.totals) {
     run();
@@ -770,7 +1004,7 @@ void run_phases(GnArgs& a, const ivid_gn_act_desc* d, int ve, const Scratch& s, 
   run();
   const dim3 grid((unsigned)((long long)d->N * a.cut.nslab));
   double2* totals = (double2*)((char*)scratch + s.words);
-#define TOTAL(VE) hipLaunchKernelGGL((gn_act_total_kernel<VE, MOMENTS>), grid, dim3(NT), 0, st, a, (const unsigned long long*)scratch, totals)
+#define TOTAL(VE) hipLaunchKernelGGL((gn_act_total_kernel<NT, VE, MOMENTS>), grid, dim3(NT), 0, st, a, (const unsigned long long*)scratch, totals)
   if (ve == 8) TOTAL(8); else if (ve == 4) TOTAL(4); else if (ve == 2) TOTAL(2); else TOTAL(1);
 #undef TOTAL
   a.cut.phase = PH_RESULT;
@@ -796,26 +1030,34 @@ extern "C" int ivid_gn_act_forward(const ivid_gn_act_desc* d, void* out, float* 
   if (int e = clear_words(s, scratch, st)) return e;
   const dim3 grid((unsigned)((long long)d->N * a.cut.nslab * a.cut.K));
 #define LAUNCH(T, VE, NV) \
-  hipLaunchKernelGGL((gn_act_fwd_kernel<T, VE, NV>), grid, dim3(NT), 0, st, a, (char*)out, stats, (unsigned long long*)scratch, \
+  hipLaunchKernelGGL((gn_act_fwd_kernel<NT_FWD, T, VE, NV>), grid, dim3(NT_FWD), 0, st, a, (char*)out, stats, (unsigned long long*)scratch, \
                      (const double2*)((char*)scratch + s.words))
-#define LAUNCH16(T)                                   \
-  do {                                                \
-    if (ve == 8) LAUNCH(T, 8, NV_FWD);                \
-    else if (ve == 4) LAUNCH(T, 4, NV_FWD);           \
-    else if (ve == 2) LAUNCH(T, 2, NV_NARROW);        \
-    else LAUNCH(T, 1, NV_NARROW);                     \
+#define LAUNCH_NV(T, VE)                                        \
+  do {                                                          \
+    if (a.cut.nv == SWEEPS_FWD[0]) LAUNCH(T, VE, SWEEPS_FWD[0]);   \
+    else if (a.cut.nv == SWEEPS_FWD[1]) LAUNCH(T, VE, SWEEPS_FWD[1]); \
+    else if (a.cut.nv == SWEEPS_FWD[2]) LAUNCH(T, VE, SWEEPS_FWD[2]); \
+    else LAUNCH(T, VE, SWEEPS_FWD[3]);                            \
   } while (0)
-  run_phases<true>(a, d, ve, s, scratch, st, [&] {
+#define LAUNCH16(T)                               \
+  do {                                            \
+    if (ve == 8) LAUNCH_NV(T, 8);                 \
+    else if (ve == 4) LAUNCH(T, 4, SWEEPS_NARROW); \
+    else if (ve == 2) LAUNCH(T, 2, SWEEPS_NARROW); \
+    else LAUNCH(T, 1, SWEEPS_NARROW);             \
+  } while (0)
+  run_phases<NT_FWD, true>(a, d, ve, s, scratch, st, [&] {
     if (d->dtype == IVID_F32) {
-      if (ve == 4) LAUNCH(float, 4, NV_FWD);
-      else if (ve == 2) LAUNCH(float, 2, NV_NARROW);
-      else LAUNCH(float, 1, NV_NARROW);
+      if (ve == 4) LAUNCH_NV(float, 4);
+      else if (ve == 2) LAUNCH(float, 2, SWEEPS_NARROW);
+      else LAUNCH(float, 1, SWEEPS_NARROW);
     } else if (d->dtype == IVID_BF16) {
       LAUNCH16(__bf16);
     } else {
       LAUNCH16(_Float16);
     }
   });
+#undef LAUNCH_NV
 #undef LAUNCH16
 #undef LAUNCH
   return ivid_check_launch("gn_act_forward");
@@ -829,7 +1071,7 @@ extern "C" int ivid_gn_act_backward(const ivid_gn_act_desc* d, const float* stat
   if (!dgamma || !dbeta || (d->C1 > 0) != (dsrc1 != nullptr) || (d->film != nullptr) != (dfilm != nullptr))
     return ivid_set_error("gn_act_backward: an output is missing or has no input", hipSuccess);
   if (!stats || !dy || !dsrc0 || (((uintptr_t)dy | (uintptr_t)dsrc0 | (uintptr_t)dsrc1) & 15) ||
-      (((uintptr_t)stats | (uintptr_t)dgamma | (uintptr_t)dbeta | (uintptr_t)dfilm) & 3))
+      ((uintptr_t)stats & 7) || (((uintptr_t)dgamma | (uintptr_t)dbeta | (uintptr_t)dfilm) & 3))
     return ivid_set_error("gn_act_backward: NULL or misaligned pointer", hipSuccess);
   const Scratch s = layout(d, a, true);
   if (scratch_bytes < s.total || !scratch || ((uintptr_t)scratch & 15)) return ivid_set_error("gn_act_backward: scratch too small or misaligned", hipSuccess);
@@ -839,34 +1081,42 @@ extern "C" int ivid_gn_act_backward(const ivid_gn_act_desc* d, const float* stat
   float2* part = (float2*)((char*)scratch + s.words + s.totals + s.ab);
   const dim3 grid((unsigned)((long long)d->N * a.cut.nslab * a.cut.K));
 #define LAUNCH(T, VE, NV)                                                                                              \
-  hipLaunchKernelGGL((gn_act_bwd_kernel<T, VE, NV>), grid, dim3(NT), 0, st, a, stats, (const char*)dy, (char*)dsrc0,   \
+  hipLaunchKernelGGL((gn_act_bwd_kernel<NT_BWD, T, VE, NV>), grid, dim3(NT_BWD), 0, st, a, stats, (const char*)dy, (char*)dsrc0,   \
                      (char*)dsrc1, (unsigned long long*)scratch, (const double2*)((char*)scratch + s.words), part, ab, (char*)dfilm)
-#define LAUNCH16(T)                                   \
-  do {                                                \
-    if (ve == 8) LAUNCH(T, 8, NV_BWD);                \
-    else if (ve == 4) LAUNCH(T, 4, NV_BWD);           \
-    else if (ve == 2) LAUNCH(T, 2, NV_NARROW);        \
-    else LAUNCH(T, 1, NV_NARROW);                     \
+#define LAUNCH_NV(T, VE)                                        \
+  do {                                                          \
+    if (a.cut.nv == SWEEPS_BWD[0]) LAUNCH(T, VE, SWEEPS_BWD[0]);   \
+    else if (a.cut.nv == SWEEPS_BWD[1]) LAUNCH(T, VE, SWEEPS_BWD[1]); \
+    else if (a.cut.nv == SWEEPS_BWD[2]) LAUNCH(T, VE, SWEEPS_BWD[2]); \
+    else LAUNCH(T, VE, SWEEPS_BWD[3]);                            \
   } while (0)
-  run_phases<false>(a, d, ve, s, scratch, st, [&] {
+#define LAUNCH16(T)                               \
+  do {                                            \
+    if (ve == 8) LAUNCH_NV(T, 8);                 \
+    else if (ve == 4) LAUNCH(T, 4, SWEEPS_NARROW); \
+    else if (ve == 2) LAUNCH(T, 2, SWEEPS_NARROW); \
+    else LAUNCH(T, 1, SWEEPS_NARROW);             \
+  } while (0)
+  run_phases<NT_BWD, false>(a, d, ve, s, scratch, st, [&] {
     if (d->dtype == IVID_F32) {
-      if (ve == 4) LAUNCH(float, 4, NV_BWD);
-      else if (ve == 2) LAUNCH(float, 2, NV_NARROW);
-      else LAUNCH(float, 1, NV_NARROW);
+      if (ve == 4) LAUNCH_NV(float, 4);
+      else if (ve == 2) LAUNCH(float, 2, SWEEPS_NARROW);
+      else LAUNCH(float, 1, SWEEPS_NARROW);
     } else if (d->dtype == IVID_BF16) {
       LAUNCH16(__bf16);
     } else {
       LAUNCH16(_Float16);
     }
   });
+#undef LAUNCH_NV
 #undef LAUNCH16
 #undef LAUNCH
   if (s.part) {
     const dim3 g2((unsigned)((long long)d->N * ((a.C + 63) / 64)));
-#define FILM(T) hipLaunchKernelGGL(gn_act_film_kernel<T>, g2, dim3(NT), 0, st, a, (const float2*)part, ab, (char*)dfilm)
+#define FILM(T) hipLaunchKernelGGL(gn_act_film_kernel<T>, g2, dim3(NT_AUX), 0, st, a, (const float2*)part, ab, (char*)dfilm)
     if (d->dtype == IVID_F32) FILM(float); else if (d->dtype == IVID_BF16) FILM(__bf16); else FILM(_Float16);
 #undef FILM
   }
-  hipLaunchKernelGGL(gn_act_param_kernel, dim3((unsigned)((a.C + 15) / 16)), dim3(NT), 0, st, (const float2*)ab, d->N, a.C, dgamma, dbeta);
+  hipLaunchKernelGGL(gn_act_param_kernel, dim3((unsigned)((a.C + 15) / 16)), dim3(NT_AUX), 0, st, (const float2*)ab, d->N, a.C, dgamma, dbeta);
   return ivid_check_launch("gn_act_backward");
 }

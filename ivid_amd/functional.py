@@ -57,23 +57,21 @@ def _check_x(x, name):
         raise _lib.IvidHipError(f"{name} is on {x.device}: ivid_amd has no CPU path")
 
 
-class _on:
-    """The tensors' device made current for the launches, when it is not."""
-
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard:
-            self.guard.__exit__(*exc)
+def _launch(name, device, *args):
+    """One library call on torch's current stream of `device`, which is made current for it when it is not."""
+    fn = getattr(_lib.load(), name)
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        _lib.check(status, name)
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _raw_stream(index):
+    return torch._C._cuda_getCurrentRawStream(index)      # torch.cuda.current_stream(index).cuda_stream without its 2 us
 
 
 def _refuse_captured_leaves(*tensors):
@@ -88,9 +86,7 @@ def _dropout(x, p, rng):
     out = torch.empty_like(x)
     if x.numel():
         seed, sid, dev = _rng_args(rng, p, x.device)
-        with _on(x.device):
-            _lib.call("ivid_dropout", _DTYPES[x.dtype], x.data_ptr(), out.data_ptr(), x.numel(), p, seed, sid, dev,
-                      _stream(x.device))
+        _launch("ivid_dropout", x.device, _DTYPES[x.dtype], x.data_ptr(), out.data_ptr(), x.numel(), p, seed, sid, dev)
     return out
 
 
@@ -149,17 +145,16 @@ def _pixels(x):
 
 
 class _Call:
-    """Checked arguments of one group_norm_act call, as the library takes them; keeps what the descriptor points to alive."""
+    """Checked arguments of one group_norm_act call, as the library takes them."""
 
     def __init__(self, x, groups, weight, bias, film, skip, act, eps, p, rng):
         _check_x(x, "x")
-        if x.dim() < 2:
+        dev, dtype, shape = x.device, x.dtype, x.shape
+        if len(shape) < 2:
             raise ValueError("x must be [N, ..., C]")
-        n, c0 = x.shape[0], x.shape[-1]
-        c1 = 0
-        dev = x.device
+        n, c0, c1 = shape[0], shape[-1], 0
         if skip is not None:
-            if skip.dtype != x.dtype or skip.device != dev or skip.shape[:-1] != x.shape[:-1]:
+            if skip.dtype != dtype or skip.device != dev or skip.shape[:-1] != shape[:-1]:
                 raise ValueError("skip must match x in everything but the number of channels")
             c1 = skip.shape[-1]
         c = c0 + c1
@@ -170,55 +165,60 @@ class _Call:
         for name, t in (("weight", weight), ("bias", bias)):
             if t.dtype != torch.float32:
                 raise TypeError(f"{name} must be float32, got {t.dtype}")
-            if t.shape != (c,) or t.device != dev:
+            if t.dim() != 1 or t.shape[0] != c or t.device != dev:
                 raise ValueError(f"{name} must be [{c}] on {dev}")
         if film is not None:
-            if film.dtype not in (torch.float32, x.dtype):
-                raise TypeError(f"film must be float32 or {x.dtype}, got {film.dtype}")
+            if film.dtype != torch.float32 and film.dtype != dtype:
+                raise TypeError(f"film must be float32 or {dtype}, got {film.dtype}")
             if film.shape != (n, 2 * c) or film.device != dev:
                 raise ValueError(f"film must be [{n}, {2 * c}] (scale, shift) on {dev}")
-            if film.stride(1) != 1:
-                film = film.contiguous()
         if act not in _ACTS:
             raise ValueError(f"act must be one of {sorted(_ACTS)}, got {act!r}")
         if not (eps > 0 and math.isfinite(eps)):
             raise ValueError(f"eps must be positive, got {eps}")
         p = _check_p(p)
-        seed, sid, rng_ptr = _rng_args(rng, p, dev)
-        self.shape = x.shape[:-1] + (c,)
-        self.device, self.dtype = dev, x.dtype
-        self.n, self.c0, self.c1, self.c, self.groups = n, c0, c1, c, groups
-        self.empty = x.numel() == 0
-        x, ld0, sn0 = _pixels(x)
+        numel = x.numel()
+        self.device, self.dtype = dev, dtype
+        self.film_dtype = film.dtype if film is not None else None
+        self.shape = shape if c1 == 0 else shape[:-1] + (c,)
+        self.n, self.c0, self.c1, self.c, self.groups, self.p = n, c0, c1, c, groups, p
+        self.empty = numel == 0
+        d = self.desc = _lib.GnActDesc(_DTYPES[dtype], n, 0 if self.empty else numel // (n * c0), c0, c1, groups, _ACTS[act])
+        d.eps, d.p, d.max_polls = eps, p, _MAX_POLLS
+        self.bind(x, weight, bias, film, skip, rng)
+
+    def bind(self, x, weight, bias, film, skip, rng):
+        """Point the descriptor at these tensors (of the shapes and types checked in front), which the caller keeps alive."""
+        d = self.desc
+        x, d.ld0, d.sn0 = _pixels(x)
         if skip is not None:
-            skip, ld1, sn1 = _pixels(skip)
-        else:
-            ld1 = sn1 = 0
+            skip, d.ld1, d.sn1 = _pixels(skip)
+            d.src1 = skip.data_ptr()
         weight, bias = weight.contiguous(), bias.contiguous()
+        d.src0, d.gamma, d.beta = x.data_ptr(), weight.data_ptr(), bias.data_ptr()
+        if film is not None:
+            if film.stride(1) != 1:
+                film = film.contiguous()
+            d.film, d.film_ld, d.film_dtype = film.data_ptr(), film.stride(0), _DTYPES[film.dtype]
+        d.seed, d.stream_id, d.rng = _rng_args(rng, self.p, self.device)
         self.keep = (x, skip, weight, bias, film, rng)
-        ptr = _lib.ptr
-        self.film = film
-        self.desc = _lib.GnActDesc(
-            _DTYPES[x.dtype], n, 0 if self.empty else x.numel() // (n * c0), c0, c1, groups, _ACTS[act],
-            x.data_ptr(), ld0, sn0, ptr(skip), ld1, sn1, weight.data_ptr(), bias.data_ptr(), ptr(film),
-            _DTYPES[film.dtype] if film is not None else 0, film.stride(0) if film is not None else 0, eps, p, seed, sid, rng_ptr,
-            _MAX_POLLS)
 
     def scratch(self, backward):
         nbytes = _lib.load().ivid_gn_act_scratch_bytes(C.byref(self.desc), backward)
-        if nbytes < 0:
-            _lib.check(-1, "ivid_gn_act_scratch_bytes")
-        return (torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None), nbytes
+        if nbytes <= 0:
+            if nbytes < 0:
+                _lib.check(-1, "ivid_gn_act_scratch_bytes")
+            return None, 0, None
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        return buf.data_ptr(), nbytes, buf
 
     def forward(self):
         y = torch.empty(self.shape, dtype=self.dtype, device=self.device)
-        stats = torch.empty(self.n, self.groups, 2, dtype=torch.float32, device=self.device)
+        stats = torch.empty((self.n, self.groups, 2), dtype=torch.float32, device=self.device)
         if self.empty:
             return y, stats.zero_()
-        with _on(self.device):
-            scratch, nbytes = self.scratch(0)
-            _lib.call("ivid_gn_act_forward", C.byref(self.desc), y.data_ptr(), stats.data_ptr(), _lib.ptr(scratch), nbytes,
-                      _stream(self.device))
+        ptr, nbytes, buf = self.scratch(0)
+        _launch("ivid_gn_act_forward", self.device, C.byref(self.desc), y.data_ptr(), stats.data_ptr(), ptr, nbytes)
         return y, stats
 
     def backward(self, dy, stats):
@@ -230,17 +230,17 @@ class _Call:
         if dy.data_ptr() % 16:
             dy = dy.clone()
         new = torch.zeros if self.empty else torch.empty
-        dev = self.device
-        dx = new(self.shape[:-1] + (self.c0,), dtype=self.dtype, device=dev)
-        dskip = new(self.shape[:-1] + (self.c1,), dtype=self.dtype, device=dev) if self.c1 else None
-        dparam = new(2, self.c, dtype=torch.float32, device=dev)
-        dfilm = new(self.n, 2 * self.c, dtype=self.film.dtype, device=dev) if self.film is not None else None
+        dev, head, c = self.device, self.shape[:-1], self.c
+        dx = new(head + (self.c0,), dtype=self.dtype, device=dev)
+        dskip = new(head + (self.c1,), dtype=self.dtype, device=dev) if self.c1 else None
+        dweight = new(c, dtype=torch.float32, device=dev)
+        dbias = new(c, dtype=torch.float32, device=dev)
+        dfilm = new((self.n, 2 * c), dtype=self.film_dtype, device=dev) if self.film_dtype is not None else None
         if not self.empty:
-            with _on(dev):
-                scratch, nbytes = self.scratch(1)
-                _lib.call("ivid_gn_act_backward", C.byref(self.desc), stats.data_ptr(), dy.data_ptr(), dx.data_ptr(), _lib.ptr(dskip),
-                          dparam.data_ptr(), dparam.data_ptr() + 4 * self.c, _lib.ptr(dfilm), _lib.ptr(scratch), nbytes, _stream(dev))
-        return dx, dskip, dparam[0], dparam[1], dfilm
+            ptr, nbytes, buf = self.scratch(1)
+            _launch("ivid_gn_act_backward", dev, C.byref(self.desc), stats.data_ptr(), dy.data_ptr(), dx.data_ptr(), _lib.ptr(dskip),
+                    dweight.data_ptr(), dbias.data_ptr(), _lib.ptr(dfilm), ptr, nbytes)
+        return dx, dskip, dweight, dbias, dfilm
 
 
 class _GroupNormAct(torch.autograd.Function):
@@ -248,17 +248,20 @@ class _GroupNormAct(torch.autograd.Function):
     def forward(ctx, x, weight, bias, film, skip, groups, act, eps, p, rng):
         call = _Call(x, groups, weight, bias, film, skip, act, eps, p, rng)
         y, stats = call.forward()
-        ctx.save_for_backward(x, weight, bias, film, skip, stats, rng if isinstance(rng, torch.Tensor) else None)
-        ctx.args = (groups, act, eps, p, rng if not isinstance(rng, torch.Tensor) else None)
+        device_rng = isinstance(rng, torch.Tensor)
+        ctx.save_for_backward(x, weight, bias, film, skip, stats, rng if device_rng else None)
+        call.keep = None        # what saves, offloads or recomputes saved tensors decides over their lives
+        ctx.call, ctx.rng = call, None if device_rng else rng
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, film, skip, stats, rng_t = ctx.saved_tensors
-        groups, act, eps, p, rng = ctx.args
-        call = _Call(x, groups, weight, bias, film, skip, act, eps, p, rng_t if rng_t is not None else rng)
+        x, weight, bias, film, skip, stats, rng = ctx.saved_tensors
+        call = ctx.call
+        call.bind(x, weight, bias, film, skip, ctx.rng if rng is None else rng)
         dx, dskip, dw, db, dfilm = call.backward(dy, stats)
+        call.keep = None
         need = ctx.needs_input_grad
         return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None, dfilm if need[3] else None,
                 dskip if need[4] else None, None, None, None, None, None)
