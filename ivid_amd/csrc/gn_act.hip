@@ -538,20 +538,6 @@ __global__ __launch_bounds__(NT, 4) void gn_act_fwd_kernel(GnArgs a, char* __res
 }
 
 // ---- backward ----
-// dscale, dshift of one (n, c) and its share of dgamma, dbeta
-template <typename T>
-__device__ __forceinline__ void channel_done(const GnArgs& a, int n, int c, float A, float B, float2* ab, char* dfilm) {
-  float gain = 1.0f;
-  if (a.film_kind) {
-    gain += film_at<T>(a, (long long)n * a.film_ld + c);
-    const float ds = __builtin_fmaf(a.gamma[c], B, a.beta[c] * A);
-    const long long i = (long long)n * 2 * a.C + c;
-    if (a.film_kind == 1) { ((float*)dfilm)[i] = ds; ((float*)dfilm)[i + a.C] = A; }
-    else { ((T*)dfilm)[i] = (T)ds; ((T*)dfilm)[i + a.C] = (T)A; }
-  }
-  ab[(long long)n * a.C + c] = make_float2(gain * A, gain * B);
-}
-
 // d: dy -> gv, f: x -> xc, of one piece; o = its index in dy
 template <int VE>
 __device__ __forceinline__ void gradient_of(const GnArgs& a, long long o, const float* m, const float* sc, const float* bb, float* f, float* d) {
@@ -673,8 +659,7 @@ __device__ __forceinline__ void help_backward(const GnArgs& a, int n, int slab, 
 template <int NT, typename T, int VE, int NV>
 __global__ __launch_bounds__(NT, 2) void gn_act_bwd_kernel(GnArgs a, const float* __restrict__ stats, const char* __restrict__ dy,
                                                            char* __restrict__ d0, char* __restrict__ d1, unsigned long long* words,
-                                                           const double2* __restrict__ totals, float2* __restrict__ part,
-                                                           float2* __restrict__ ab, char* __restrict__ dfilm) {
+                                                           const double2* __restrict__ totals, float2* __restrict__ part) {
   typedef typename Piece<T, VE>::reg reg_t;
   typedef typename Piece<T, VE>::mem mem_t;
   __shared__ __attribute__((aligned(16))) float redA[NT * (VE + 8)], redB[NT * (VE + 8)];
@@ -747,8 +732,7 @@ __global__ __launch_bounds__(NT, 2) void gn_act_bwd_kernel(GnArgs a, const float
       left -= q.RPI;
     });
     join_gradients<NT, VE>(a, t, slab, A, B, h, [&](int j, float sa, float sb) __attribute__((always_inline)) {
-      if (q.krows > 1) part[((size_t)n * q.krows + (q.kcols > 1 ? me / q.kcols : me)) * a.C + t.cb + j] = make_float2(sa, sb);
-      else channel_done<T>(a, n, t.cb + j, sa, sb, ab, dfilm);
+      part[((size_t)n * q.krows + (q.kcols > 1 ? me / q.kcols : me)) * a.C + t.cb + j] = make_float2(sa, sb);
     });
   }
   const float Mf = (float)a.HW * (float)a.Cg;
@@ -836,37 +820,16 @@ __global__ __launch_bounds__(NT_AUX) void gn_act_clear_kernel(ulonglong2* words,
   if (i < n) words[i] = make_ulonglong2(0, 0);
 }
 
-// part [N][krows][C] -> ab [N][C], dfilm: 64 channels a workgroup, four threads a channel
-template <typename T>
-__global__ __launch_bounds__(NT_AUX) void gn_act_film_kernel(GnArgs a, const float2* __restrict__ part, float2* __restrict__ ab, char* __restrict__ dfilm) {
+// part [N][krows][C] -> [N][1][C]: 64 channels a workgroup, four threads a channel
+__global__ __launch_bounds__(NT_AUX) void gn_act_fold_kernel(const float2* __restrict__ part, int krows, int C, float2* __restrict__ out) {
   __shared__ float2 red[NT_AUX];
-  const int cblk = (a.C + 63) / 64;
+  const int cblk = (C + 63) / 64;
   const int n = blockIdx.x / cblk, c = (blockIdx.x - n * cblk) * 64 + (threadIdx.x & 63), h = threadIdx.x >> 6;
   float A = 0.f, B = 0.f;
-  if (c < a.C) {
-    for (int k = h; k < a.cut.krows; k += NT_AUX / 64) {
-      const float2 v = part[((size_t)n * a.cut.krows + k) * a.C + c];
-      A += v.x;
-      B += v.y;
-    }
-  }
-  red[threadIdx.x] = make_float2(A, B);
-  __syncthreads();
-  if (h == 0 && c < a.C) {
-#pragma unroll
-    for (int j = 1; j < NT_AUX / 64; ++j) { A += red[threadIdx.x + 64 * j].x; B += red[threadIdx.x + 64 * j].y; }
-    channel_done<T>(a, n, c, A, B, ab, dfilm);
-  }
-}
-
-// ab [N][C] -> dgamma, dbeta: 16 channels a workgroup, 16 threads a channel
-__global__ __launch_bounds__(NT_AUX) void gn_act_param_kernel(const float2* __restrict__ ab, int N, int C, float* __restrict__ dgamma, float* __restrict__ dbeta) {
-  __shared__ float2 red[NT_AUX];
-  const int c = blockIdx.x * 16 + (threadIdx.x & 15), h = threadIdx.x >> 4;
-  float A = 0.f, B = 0.f;
   if (c < C) {
-    for (int n = h; n < N; n += 16) {
-      const float2 v = ab[(size_t)n * C + c];
+#pragma unroll 4
+    for (int k = h; k < krows; k += NT_AUX / 64) {
+      const float2 v = part[((size_t)n * krows + k) * C + c];
       A += v.x;
       B += v.y;
     }
@@ -875,9 +838,48 @@ __global__ __launch_bounds__(NT_AUX) void gn_act_param_kernel(const float2* __re
   __syncthreads();
   if (h == 0 && c < C) {
 #pragma unroll
-    for (int j = 1; j < 16; ++j) { A += red[threadIdx.x + 16 * j].x; B += red[threadIdx.x + 16 * j].y; }
-    dgamma[c] = B;
-    dbeta[c] = A;
+    for (int j = 1; j < NT_AUX / 64; ++j) { A += red[threadIdx.x + 64 * j].x; B += red[threadIdx.x + 64 * j].y; }
+    out[(size_t)n * C + c] = make_float2(A, B);
+  }
+}
+
+// part [N][krows][C] (A, B of a tile) -> dscale, dshift of every (n, c), dgamma, dbeta: 16 channels a workgroup, 16 threads a channel
+template <typename T>
+__global__ __launch_bounds__(NT_AUX) void gn_act_param_kernel(GnArgs a, const float2* __restrict__ part, int krows, int N, float* __restrict__ dgamma,
+                                                              float* __restrict__ dbeta, char* __restrict__ dfilm) {
+  __shared__ float2 red[NT_AUX];
+  const int c = blockIdx.x * 16 + (threadIdx.x & 15), h = threadIdx.x >> 4;
+  float sa = 0.f, sb = 0.f;
+  if (c < a.C) {
+    const float gamma = a.gamma[c], beta = a.beta[c];
+    for (int n = h; n < N; n += 16) {
+      float A = 0.f, B = 0.f;
+      const float2* p = part + (size_t)n * krows * a.C + c;
+#pragma unroll 4
+      for (int k = 0; k < krows; ++k) {
+        const float2 v = p[(size_t)k * a.C];
+        A += v.x;
+        B += v.y;
+      }
+      float gain = 1.0f;
+      if (a.film_kind) {
+        gain += film_at<T>(a, (long long)n * a.film_ld + c);
+        const float ds = __builtin_fmaf(gamma, B, beta * A);
+        const long long i = (long long)n * 2 * a.C + c;
+        if (a.film_kind == 1) { ((float*)dfilm)[i] = ds; ((float*)dfilm)[i + a.C] = A; }
+        else { ((T*)dfilm)[i] = (T)ds; ((T*)dfilm)[i + a.C] = (T)A; }
+      }
+      sa = __builtin_fmaf(gain, A, sa);
+      sb = __builtin_fmaf(gain, B, sb);
+    }
+  }
+  red[threadIdx.x] = make_float2(sa, sb);
+  __syncthreads();
+  if (h == 0 && c < a.C) {
+#pragma unroll
+    for (int j = 1; j < 16; ++j) { sa += red[threadIdx.x + 16 * j].x; sb += red[threadIdx.x + 16 * j].y; }
+    dgamma[c] = sb;
+    dbeta[c] = sa;
   }
 }
 
@@ -970,18 +972,22 @@ int fill_args(const ivid_gn_act_desc* d, bool backward, GnArgs* a, int* ve) {
   return cut_up(d, backward, a, ve);
 }
 
-// scratch: the clusters' words, (K > MAX_K) their totals, then (backward) ab [N][C] and part [N][krows][C]
-struct Scratch { long long words, totals, ab, part, total; };
+// The channels' sums take a launch of their own over the tiles before they are added over the samples when one thread would walk over
+// more tiles than this (three microseconds of it cost as much as the launch).
+constexpr int FOLD_ABOVE = 48;
+
+// scratch: the clusters' words, (K > MAX_K) their totals, then (backward) part [N][krows][C] and, if folded, part [N][C]
+struct Scratch { long long words, totals, part, folded, total; };
 Scratch layout(const ivid_gn_act_desc* d, const GnArgs& a, bool backward) {
   Scratch s{};
   const Cut& q = a.cut;
   if (q.K > 1) s.words = (long long)d->N * q.nslab * q.K * q.GS * 16;
   if (q.K > MAX_K) s.totals = (long long)d->N * q.nslab * q.GS * 16;
   if (backward) {
-    s.ab = (long long)d->N * a.C * 8;
-    if (q.krows > 1) s.part = (long long)d->N * q.krows * a.C * 8;
+    s.part = (long long)d->N * q.krows * a.C * 8;
+    if (q.krows > 1 && (long long)q.krows * ((d->N + 15) / 16) > FOLD_ABOVE) s.folded = (long long)d->N * a.C * 8;
   }
-  s.total = s.words + s.totals + s.ab + s.part;
+  s.total = s.words + s.totals + s.part + s.folded;
   return s;
 }
 
@@ -1077,12 +1083,11 @@ extern "C" int ivid_gn_act_backward(const ivid_gn_act_desc* d, const float* stat
   if (scratch_bytes < s.total || !scratch || ((uintptr_t)scratch & 15)) return ivid_set_error("gn_act_backward: scratch too small or misaligned", hipSuccess);
   hipStream_t st = (hipStream_t)stream;
   if (int e = clear_words(s, scratch, st)) return e;
-  float2* ab = (float2*)((char*)scratch + s.words + s.totals);
-  float2* part = (float2*)((char*)scratch + s.words + s.totals + s.ab);
+  float2* part = (float2*)((char*)scratch + s.words + s.totals);
   const dim3 grid((unsigned)((long long)d->N * a.cut.nslab * a.cut.K));
 #define LAUNCH(T, VE, NV)                                                                                              \
   hipLaunchKernelGGL((gn_act_bwd_kernel<NT_BWD, T, VE, NV>), grid, dim3(NT_BWD), 0, st, a, stats, (const char*)dy, (char*)dsrc0,   \
-                     (char*)dsrc1, (unsigned long long*)scratch, (const double2*)((char*)scratch + s.words), part, ab, (char*)dfilm)
+                     (char*)dsrc1, (unsigned long long*)scratch, (const double2*)((char*)scratch + s.words), part)
 #define LAUNCH_NV(T, VE)                                        \
   do {                                                          \
     if (a.cut.nv == SWEEPS_BWD[0]) LAUNCH(T, VE, SWEEPS_BWD[0]);   \
@@ -1111,12 +1116,17 @@ extern "C" int ivid_gn_act_backward(const ivid_gn_act_desc* d, const float* stat
 #undef LAUNCH_NV
 #undef LAUNCH16
 #undef LAUNCH
-  if (s.part) {
-    const dim3 g2((unsigned)((long long)d->N * ((a.C + 63) / 64)));
-#define FILM(T) hipLaunchKernelGGL(gn_act_film_kernel<T>, g2, dim3(NT_AUX), 0, st, a, (const float2*)part, ab, (char*)dfilm)
-    if (d->dtype == IVID_F32) FILM(float); else if (d->dtype == IVID_BF16) FILM(__bf16); else FILM(_Float16);
-#undef FILM
+  int krows = a.cut.krows;
+  if (s.folded) {
+    float2* folded = (float2*)((char*)part + s.part);
+    hipLaunchKernelGGL(gn_act_fold_kernel, dim3((unsigned)((long long)d->N * ((a.C + 63) / 64))), dim3(NT_AUX), 0, st, (const float2*)part, krows, a.C, folded);
+    part = folded;
+    krows = 1;
   }
-  hipLaunchKernelGGL(gn_act_param_kernel, dim3((unsigned)((a.C + 15) / 16)), dim3(NT_AUX), 0, st, (const float2*)ab, d->N, a.C, dgamma, dbeta);
+#define PARAM(T)                                                                                                                    \
+  hipLaunchKernelGGL(gn_act_param_kernel<T>, dim3((unsigned)((a.C + 15) / 16)), dim3(NT_AUX), 0, st, a, (const float2*)part, krows, \
+                     d->N, dgamma, dbeta, (char*)dfilm)
+  if (d->dtype == IVID_F32) PARAM(float); else if (d->dtype == IVID_BF16) PARAM(__bf16); else PARAM(_Float16);
+#undef PARAM
   return ivid_check_launch("gn_act_backward");
 }

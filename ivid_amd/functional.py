@@ -20,6 +20,7 @@ import ctypes as C
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -57,21 +58,23 @@ def _check_x(x, name):
         raise _lib.IvidHipError(f"{name} is on {x.device}: ivid_amd has no CPU path")
 
 
+_entry = {}     # the library's entry points by name
+
+
 def _launch(name, device, *args):
     """One library call on torch's current stream of `device`, which is made current for it when it is not."""
-    fn = getattr(_lib.load(), name)
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(_lib.load(), name)
     index = device.index
+    # (the raw getter is torch.cuda.current_stream(index).cuda_stream without its 2 us)
     if index == torch.cuda.current_device():
-        status = fn(*args, _raw_stream(index))
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            status = fn(*args, _raw_stream(index))
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         _lib.check(status, name)
-
-
-def _raw_stream(index):
-    return torch._C._cuda_getCurrentRawStream(index)      # torch.cuda.current_stream(index).cuda_stream without its 2 us
 
 
 def _refuse_captured_leaves(*tensors):
@@ -82,12 +85,24 @@ def _refuse_captured_leaves(*tensors):
 
 # ---- dropout ----
 def _dropout(x, p, rng):
-    x = x.contiguous()
+    if not x.is_contiguous():
+        x = x.contiguous()
     out = torch.empty_like(x)
-    if x.numel():
-        seed, sid, dev = _rng_args(rng, p, x.device)
-        _launch("ivid_dropout", x.device, _DTYPES[x.dtype], x.data_ptr(), out.data_ptr(), x.numel(), p, seed, sid, dev)
+    n = x.numel()
+    if n:
+        device = x.device
+        seed, sid, dev = _rng_args(rng, p, device)
+        _launch("ivid_dropout", device, _DTYPES[x.dtype], x.data_ptr(), out.data_ptr(), n, p, seed, sid, dev)
     return out
+
+
+# The backward passes run in autograd's own thread, where Python is several times slower than in the caller's: what can be prepared in
+# the forward call is, and the wrapper that makes them differentiable once is only entered under create_graph.
+def _dropout_grads(ctx, dy):
+    return _dropout(dy, ctx.p, ctx.saved_tensors[0] if ctx.rng is None else ctx.rng), None, None
+
+
+_dropout_grads_once = once_differentiable(_dropout_grads)
 
 
 class _Dropout(torch.autograd.Function):
@@ -100,9 +115,8 @@ class _Dropout(torch.autograd.Function):
         return _dropout(x, p, rng)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        return _dropout(dy, ctx.p, ctx.saved_tensors[0] if ctx.saved_tensors else ctx.rng), None, None
+        return _dropout_grads_once(ctx, dy) if torch.is_grad_enabled() else _dropout_grads(ctx, dy)
 
 
 def dropout(x, p, rng=None):
@@ -113,7 +127,6 @@ def dropout(x, p, rng=None):
     gradient by hand, call it on the gradient with the same rng: the operator is its own backward pass."""
     _check_x(x, "x")
     p = _check_p(p)
-    _rng_args(rng, p, x.device)
     if torch.is_grad_enabled() and x.requires_grad:
         _refuse_captured_leaves(x)
         return _Dropout.apply(x, p, rng)
@@ -183,6 +196,7 @@ class _Call:
         self.shape = shape if c1 == 0 else shape[:-1] + (c,)
         self.n, self.c0, self.c1, self.c, self.groups, self.p = n, c0, c1, c, groups, p
         self.empty = numel == 0
+        self.backward_bytes = None
         d = self.desc = _lib.GnActDesc(_DTYPES[dtype], n, 0 if self.empty else numel // (n * c0), c0, c1, groups, _ACTS[act])
         d.eps, d.p, d.max_polls = eps, p, _MAX_POLLS
         self.bind(x, weight, bias, film, skip, rng)
@@ -190,6 +204,10 @@ class _Call:
     def bind(self, x, weight, bias, film, skip, rng):
         """Point the descriptor at these tensors (of the shapes and types checked in front), which the caller keeps alive."""
         d = self.desc
+        self.strides = (x.stride(), weight.stride(), bias.stride(), None if film is None else film.stride(),
+                        None if skip is None else skip.stride())
+        self.in_place = (x.is_contiguous() and weight.is_contiguous() and bias.is_contiguous()
+                         and (film is None or film.is_contiguous()) and (skip is None or skip.is_contiguous()))
         x, d.ld0, d.sn0 = _pixels(x)
         if skip is not None:
             skip, d.ld1, d.sn1 = _pixels(skip)
@@ -203,11 +221,33 @@ class _Call:
         d.seed, d.stream_id, d.rng = _rng_args(rng, self.p, self.device)
         self.keep = (x, skip, weight, bias, film, rng)
 
+    def rebind(self, x, weight, bias, film, skip, rng):
+        """bind() for the tensors that autograd saved, which are mostly where they were."""
+        if self.in_place and self.strides == (x.stride(), weight.stride(), bias.stride(), None if film is None else film.stride(),
+                                              None if skip is None else skip.stride()):
+            d = self.desc
+            d.src0, d.gamma, d.beta = x.data_ptr(), weight.data_ptr(), bias.data_ptr()
+            if film is not None:
+                d.film = film.data_ptr()
+            if skip is not None:
+                d.src1 = skip.data_ptr()
+            if d.rng:
+                d.rng = rng.data_ptr()
+        else:
+            self.bind(x, weight, bias, film, skip, rng)
+
+    def scratch_bytes(self, backward):
+        fn = _entry.get("scratch")
+        if fn is None:
+            fn = _entry["scratch"] = _lib.load().ivid_gn_act_scratch_bytes
+        nbytes = fn(C.byref(self.desc), backward)
+        if nbytes < 0:
+            _lib.check(-1, "ivid_gn_act_scratch_bytes")
+        return nbytes
+
     def scratch(self, backward):
-        nbytes = _lib.load().ivid_gn_act_scratch_bytes(C.byref(self.desc), backward)
-        if nbytes <= 0:
-            if nbytes < 0:
-                _lib.check(-1, "ivid_gn_act_scratch_bytes")
+        nbytes = self.backward_bytes if backward and self.backward_bytes is not None else self.scratch_bytes(backward)
+        if nbytes == 0:
             return None, 0, None
         buf = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         return buf.data_ptr(), nbytes, buf
@@ -226,21 +266,53 @@ class _Call:
             raise ValueError(f"dy must be {tuple(self.shape)} {self.dtype} on {self.device}")
         if stats.shape != (self.n, self.groups, 2) or stats.dtype != torch.float32 or stats.device != self.device:
             raise ValueError("stats must be what the forward call returned")
-        dy, stats = dy.contiguous(), stats.contiguous()
+        x, skip, weight, bias, film, _ = self.keep
+        return self.gradients(dy, stats.contiguous(), x, weight, bias, film, skip)
+
+    def gradients(self, dy, stats, x, weight, bias, film, skip):
+        if not dy.is_contiguous():
+            dy = dy.contiguous()
         if dy.data_ptr() % 16:
             dy = dy.clone()
-        new = torch.zeros if self.empty else torch.empty
-        dev, head, c = self.device, self.shape[:-1], self.c
-        dx = new(head + (self.c0,), dtype=self.dtype, device=dev)
-        dskip = new(head + (self.c1,), dtype=self.dtype, device=dev) if self.c1 else None
-        dweight = new(c, dtype=torch.float32, device=dev)
-        dbias = new(c, dtype=torch.float32, device=dev)
-        dfilm = new((self.n, 2 * c), dtype=self.film_dtype, device=dev) if self.film_dtype is not None else None
-        if not self.empty:
-            ptr, nbytes, buf = self.scratch(1)
-            _launch("ivid_gn_act_backward", dev, C.byref(self.desc), stats.data_ptr(), dy.data_ptr(), dx.data_ptr(), _lib.ptr(dskip),
-                    dweight.data_ptr(), dbias.data_ptr(), _lib.ptr(dfilm), ptr, nbytes)
+        dev = self.device
+        dskip = dfilm = None
+        if self.in_place and not self.empty:
+            like = torch.empty_like
+            dx, dweight, dbias = like(x), like(weight), like(bias)
+            if skip is not None:
+                dskip = like(skip)
+            if film is not None:
+                dfilm = like(film)
+        else:
+            new = torch.zeros if self.empty else torch.empty
+            dx = new(self.shape[:-1] + (self.c0,), dtype=self.dtype, device=dev)
+            dweight = new(self.c, dtype=torch.float32, device=dev)
+            dbias = new(self.c, dtype=torch.float32, device=dev)
+            if skip is not None:
+                dskip = new(self.shape[:-1] + (self.c1,), dtype=self.dtype, device=dev)
+            if film is not None:
+                dfilm = new((self.n, 2 * self.c), dtype=self.film_dtype, device=dev)
+            if self.empty:
+                return dx, dskip, dweight, dbias, dfilm
+        ptr, nbytes, buf = self.scratch(1)
+        _launch("ivid_gn_act_backward", dev, C.byref(self.desc), stats.data_ptr(), dy.data_ptr(), dx.data_ptr(),
+                None if dskip is None else dskip.data_ptr(), dweight.data_ptr(), dbias.data_ptr(),
+                None if dfilm is None else dfilm.data_ptr(), ptr, nbytes)
         return dx, dskip, dweight, dbias, dfilm
+
+
+def _gn_grads(ctx, dy):
+    x, weight, bias, film, skip, stats, rng = ctx.saved_tensors
+    call = ctx.call
+    call.rebind(x, weight, bias, film, skip, ctx.rng if rng is None else rng)
+    dx, dskip, dw, db, dfilm = call.gradients(dy, stats, x, weight, bias, film, skip)
+    call.keep = None
+    need = ctx.needs_input_grad
+    return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None, dfilm if need[3] else None,
+            dskip if need[4] else None, None, None, None, None, None)
+
+
+_gn_grads_once = once_differentiable(_gn_grads)
 
 
 class _GroupNormAct(torch.autograd.Function):
@@ -251,20 +323,14 @@ class _GroupNormAct(torch.autograd.Function):
         device_rng = isinstance(rng, torch.Tensor)
         ctx.save_for_backward(x, weight, bias, film, skip, stats, rng if device_rng else None)
         call.keep = None        # what saves, offloads or recomputes saved tensors decides over their lives
+        if not call.empty:
+            call.backward_bytes = call.scratch_bytes(1)
         ctx.call, ctx.rng = call, None if device_rng else rng
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, film, skip, stats, rng = ctx.saved_tensors
-        call = ctx.call
-        call.bind(x, weight, bias, film, skip, ctx.rng if rng is None else rng)
-        dx, dskip, dw, db, dfilm = call.backward(dy, stats)
-        call.keep = None
-        need = ctx.needs_input_grad
-        return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None, dfilm if need[3] else None,
-                dskip if need[4] else None, None, None, None, None, None)
+        return _gn_grads_once(ctx, dy) if torch.is_grad_enabled() else _gn_grads(ctx, dy)
 
 
 def group_norm_act(x, groups, weight, bias, film=None, skip=None, act="silu", eps=1e-5, p=0.0, rng=None):
