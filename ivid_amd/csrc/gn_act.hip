@@ -33,6 +33,7 @@ constexpr int MAX_GS = 64;        // groups of a slab: at least four lanes each 
 constexpr int MAX_COL = 1024;     // channels of a tile
 constexpr int MAX_POLLS = 512;    // ~ 1 ms
 constexpr int MAX_K = 128;        // tiles of a cluster that runs as one launch
+constexpr int MIN_TILES = 16;     // of a sample, once it is cut
 enum { PH_ALL = 0, PH_SUMS = 1, PH_RESULT = 2 };
 
 // A piece of VE elements as it is kept in registers: 32-bit words.
@@ -891,14 +892,17 @@ Div div_by(int d) {
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 // Sweeps that a tile may have (instantiations): 16-byte pieces take the smallest count that holds a sample's pixels, else the largest.
-constexpr int SWEEPS_FWD[] = {2, 4, 8, 16}, SWEEPS_BWD[] = {2, 4, 8, 12}, SWEEPS_NARROW = 16;
+// Narrower pieces have two.
+constexpr int SWEEPS_FWD[] = {2, 4, 8, 16}, SWEEPS_BWD[] = {2, 4, 8, 12}, SWEEPS_NARROW[] = {4, 16};
 int sweeps_for(int ve, int esz, bool backward, long long needed) {
-  if (ve * esz < 16) return SWEEPS_NARROW;
+  if (ve * esz < 16) return SWEEPS_NARROW[needed > SWEEPS_NARROW[0]];
   const int* list = backward ? SWEEPS_BWD : SWEEPS_FWD;
   int i = 0;
   while (i < 3 && list[i] < needed) ++i;
   return list[i];
 }
+
+constexpr double TILES_COST = 2.2, SETUP_SWEEPS = 3.0;      // prices of the choice below, from measurements at 8 x 8 .. 128 x 128 pixels
 
 int cut_up(const ivid_gn_act_desc* d, bool backward, GnArgs* a, int* ve_out) {
   const int NT = backward ? NT_BWD : NT_FWD;
@@ -915,12 +919,24 @@ int cut_up(const ivid_gn_act_desc* d, bool backward, GnArgs* a, int* ve_out) {
   const int C = a->C, Cg = a->Cg;
   const long long unit = (long long)Cg / gcd(Cg, ve) * ve;     // whole groups and whole pieces
   Cut& q = a->cut;
+  // The slab: whole groups, a few whole 128-byte lines of channels.  Each candidate costs the lines that two slabs share (half of their
+  // traffic: the second reader mostly finds them in the last-level cache), the threads that have no piece, a workgroup's setup, worth
+  // about three sweeps, and, when a tile does not hold a sample's pixels, the exchange between tiles.
   long long S = unit;
-  while (S < C && S * esz < 128 && (S + unit) / Cg <= MAX_GS && (S + unit) / ve <= wide) S += unit;
-  // whole 128-byte lines, if a few more groups make them
-  for (long long s = S; s <= 4 * S && s <= C && s / Cg <= MAX_GS && s / ve <= wide; s += unit)
-    if (s * esz % 128 == 0) { S = s; break; }
-  if (S > C) S = C;            // C is a multiple of the unit
+  double best = 1e30;
+  for (long long s = unit; s <= C && (s == unit || (s / Cg <= MAX_GS && s / ve <= wide && s * esz <= 512)); s += unit) {
+    const long long pp = s / ve < wide ? s / ve : wide, rpi = NT / pp;
+    const int g = gcd((int)(s * esz % 128), 128);
+    const double lines = s == C ? 1.0 : 1.0 + (128.0 - g) / (double)(s * esz);
+    const double idle = (double)NT / (double)(pp * rpi);
+    const long long sweeps = (d->HW + rpi - 1) / rpi;
+    const double setup = 1.0 + SETUP_SWEEPS / sweeps_for(ve, esz, backward, sweeps);
+    const double cost = (0.5 + 0.5 * lines) * idle * setup * (sweeps > sweeps_for(ve, esz, backward, sweeps) ? TILES_COST : 1.0) * (s * esz < 128 && s < C ? 1.5 : 1.0);
+    if (cost < best * 0.999) {
+      best = cost;
+      S = s;
+    }
+  }
   q.S = (int)S;
   q.nslab = (int)((C + S - 1) / S);
   q.GS = (int)(S / Cg);
@@ -935,6 +951,13 @@ int cut_up(const ivid_gn_act_desc* d, bool backward, GnArgs* a, int* ve_out) {
   q.nv = sweeps_for(ve, esz, backward, ((long long)d->HW + q.RPI - 1) / q.RPI);
   q.rows = q.RPI * q.nv;
   q.krows = (int)(((long long)d->HW + q.rows - 1) / q.rows);
+  if (q.krows > 1 && (long long)q.nslab * q.krows * q.kcols < MIN_TILES && q.nv > 4) {
+    // a cluster anyway, and so few tiles that most of the chip would stand idle for a sample or two: four sweeps a tile.  (By the sample
+    // alone: its result does not depend on the batch.)
+    q.nv = 4;
+    q.rows = q.RPI * q.nv;
+    q.krows = (int)(((long long)d->HW + q.rows - 1) / q.rows);
+  }
   q.polls = d->max_polls > 0 ? d->max_polls : MAX_POLLS;
   *ve_out = ve;
   const double tiles = (double)d->N * q.nslab * q.krows * q.kcols;
@@ -1045,18 +1068,23 @@ extern "C" int ivid_gn_act_forward(const ivid_gn_act_desc* d, void* out, float* 
     else if (a.cut.nv == SWEEPS_FWD[2]) LAUNCH(T, VE, SWEEPS_FWD[2]); \
     else LAUNCH(T, VE, SWEEPS_FWD[3]);                            \
   } while (0)
+#define LAUNCH_NARROW(T, VE)                                    \
+  do {                                                          \
+    if (a.cut.nv == SWEEPS_NARROW[0]) LAUNCH(T, VE, SWEEPS_NARROW[0]); \
+    else LAUNCH(T, VE, SWEEPS_NARROW[1]);                        \
+  } while (0)
 #define LAUNCH16(T)                               \
   do {                                            \
     if (ve == 8) LAUNCH_NV(T, 8);                 \
-    else if (ve == 4) LAUNCH(T, 4, SWEEPS_NARROW); \
-    else if (ve == 2) LAUNCH(T, 2, SWEEPS_NARROW); \
-    else LAUNCH(T, 1, SWEEPS_NARROW);             \
+    else if (ve == 4) LAUNCH_NARROW(T, 4);        \
+    else if (ve == 2) LAUNCH_NARROW(T, 2);        \
+    else LAUNCH_NARROW(T, 1);                     \
   } while (0)
   run_phases<NT_FWD, true>(a, d, ve, s, scratch, st, [&] {
     if (d->dtype == IVID_F32) {
       if (ve == 4) LAUNCH_NV(float, 4);
-      else if (ve == 2) LAUNCH(float, 2, SWEEPS_NARROW);
-      else LAUNCH(float, 1, SWEEPS_NARROW);
+      else if (ve == 2) LAUNCH_NARROW(float, 2);
+      else LAUNCH_NARROW(float, 1);
     } else if (d->dtype == IVID_BF16) {
       LAUNCH16(__bf16);
     } else {
@@ -1064,6 +1092,7 @@ extern "C" int ivid_gn_act_forward(const ivid_gn_act_desc* d, void* out, float* 
     }
   });
 #undef LAUNCH_NV
+#undef LAUNCH_NARROW
 #undef LAUNCH16
 #undef LAUNCH
   return ivid_check_launch("gn_act_forward");
@@ -1095,18 +1124,23 @@ extern "C" int ivid_gn_act_backward(const ivid_gn_act_desc* d, const float* stat
     else if (a.cut.nv == SWEEPS_BWD[2]) LAUNCH(T, VE, SWEEPS_BWD[2]); \
     else LAUNCH(T, VE, SWEEPS_BWD[3]);                            \
   } while (0)
+#define LAUNCH_NARROW(T, VE)                                    \
+  do {                                                          \
+    if (a.cut.nv == SWEEPS_NARROW[0]) LAUNCH(T, VE, SWEEPS_NARROW[0]); \
+    else LAUNCH(T, VE, SWEEPS_NARROW[1]);                        \
+  } while (0)
 #define LAUNCH16(T)                               \
   do {                                            \
     if (ve == 8) LAUNCH_NV(T, 8);                 \
-    else if (ve == 4) LAUNCH(T, 4, SWEEPS_NARROW); \
-    else if (ve == 2) LAUNCH(T, 2, SWEEPS_NARROW); \
-    else LAUNCH(T, 1, SWEEPS_NARROW);             \
+    else if (ve == 4) LAUNCH_NARROW(T, 4);        \
+    else if (ve == 2) LAUNCH_NARROW(T, 2);        \
+    else LAUNCH_NARROW(T, 1);                     \
   } while (0)
   run_phases<NT_BWD, false>(a, d, ve, s, scratch, st, [&] {
     if (d->dtype == IVID_F32) {
       if (ve == 4) LAUNCH_NV(float, 4);
-      else if (ve == 2) LAUNCH(float, 2, SWEEPS_NARROW);
-      else LAUNCH(float, 1, SWEEPS_NARROW);
+      else if (ve == 2) LAUNCH_NARROW(float, 2);
+      else LAUNCH_NARROW(float, 1);
     } else if (d->dtype == IVID_BF16) {
       LAUNCH16(__bf16);
     } else {
@@ -1114,6 +1148,7 @@ extern "C" int ivid_gn_act_backward(const ivid_gn_act_desc* d, const float* stat
     }
   });
 #undef LAUNCH_NV
+#undef LAUNCH_NARROW
 #undef LAUNCH16
 #undef LAUNCH
   int krows = a.cut.krows;
