@@ -32,7 +32,9 @@ constexpr int NT_FWD = 512, NT_BWD = 256, NT_AUX = 256;
 constexpr int MAX_GS = 64;        // groups of a slab: at least four lanes each in the reductions
 constexpr int MAX_COL = 1024;     // channels of a tile
 constexpr int MAX_POLLS = 512;    // ~ 1 ms
-constexpr int MAX_K = 128;        // tiles of a cluster that runs as one launch
+// Tiles of a cluster that runs as one launch: half of the 512 workgroups of a backward pass that the chip holds at once.  8 x 256 x 256 x
+// 128 bf16, one launch against two: backward (171 tiles) 134 us against 151, forward (64 tiles) 63 against 84.
+constexpr int MAX_K = 256;
 constexpr int MIN_TILES = 16;     // of a sample, once it is cut
 enum { PH_ALL = 0, PH_SUMS = 1, PH_RESULT = 2 };
 
@@ -88,7 +90,7 @@ __device__ __forceinline__ void sweeps(F f) { sweeps_of(f, std::make_integer_seq
 
 // n / d for n < 2^24 as a multiplication: the kernels divide by run-time sizes in front of their first load
 struct Div {
-  uint32_t d, m, s;
+  uint32_t m, s;
   __device__ __forceinline__ int of(int n) const { return (int)(((uint64_t)(uint32_t)n * m) >> s); }
 };
 
@@ -844,16 +846,18 @@ __global__ __launch_bounds__(NT_AUX) void gn_act_fold_kernel(const float2* __res
   }
 }
 
-// part [N][krows][C] (A, B of a tile) -> dscale, dshift of every (n, c), dgamma, dbeta: 16 channels a workgroup, 16 threads a channel
+// part [N][krows][C] (A, B of a tile) -> dscale, dshift of every (n, c), dgamma, dbeta: 16 channels a workgroup, 16 threads a channel.
+// Workgroup row blockIdx.y takes samples [y * per, (y + 1) * per) and leaves its sums in dgamma[y][C], dbeta[y][C].
 template <typename T>
-__global__ __launch_bounds__(NT_AUX) void gn_act_param_kernel(GnArgs a, const float2* __restrict__ part, int krows, int N, float* __restrict__ dgamma,
-                                                              float* __restrict__ dbeta, char* __restrict__ dfilm) {
+__global__ __launch_bounds__(NT_AUX) void gn_act_param_kernel(GnArgs a, const float2* __restrict__ part, int krows, int N, int per,
+                                                              float* __restrict__ dgamma, float* __restrict__ dbeta, char* __restrict__ dfilm) {
   __shared__ float2 red[NT_AUX];
   const int c = blockIdx.x * 16 + (threadIdx.x & 15), h = threadIdx.x >> 4;
   float sa = 0.f, sb = 0.f;
   if (c < a.C) {
     const float gamma = a.gamma[c], beta = a.beta[c];
-    for (int n = h; n < N; n += 16) {
+    const int n1 = min(N, (int)(blockIdx.y + 1) * per);
+    for (int n = blockIdx.y * per + h; n < n1; n += 16) {
       float A = 0.f, B = 0.f;
       const float2* p = part + (size_t)n * krows * a.C + c;
 #pragma unroll 4
@@ -879,15 +883,29 @@ __global__ __launch_bounds__(NT_AUX) void gn_act_param_kernel(GnArgs a, const fl
   if (h == 0 && c < a.C) {
 #pragma unroll
     for (int j = 1; j < 16; ++j) { sa += red[threadIdx.x + 16 * j].x; sb += red[threadIdx.x + 16 * j].y; }
-    dgamma[c] = sb;
-    dbeta[c] = sa;
+    dgamma[(size_t)blockIdx.y * a.C + c] = sb;
+    dbeta[(size_t)blockIdx.y * a.C + c] = sa;
   }
+}
+// the rows of the kernel above added up
+__global__ __launch_bounds__(NT_AUX) void gn_act_rows_kernel(const float* __restrict__ g, const float* __restrict__ b, int rows, int C,
+                                                             float* __restrict__ dgamma, float* __restrict__ dbeta) {
+  const int c = blockIdx.x * NT_AUX + threadIdx.x;
+  if (c >= C) return;
+  float sa = 0.f, sb = 0.f;
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r) {
+    sb += g[(size_t)r * C + c];
+    sa += b[(size_t)r * C + c];
+  }
+  dgamma[c] = sb;
+  dbeta[c] = sa;
 }
 
 Div div_by(int d) {
   int l = 0;
   while ((1ll << l) < d) ++l;
-  return Div{(uint32_t)d, (uint32_t)(((1ull << (24 + l)) + d - 1) / d), (uint32_t)(24 + l)};
+  return Div{(uint32_t)(((1ull << (24 + l)) + d - 1) / d), (uint32_t)(24 + l)};
 }
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
@@ -998,9 +1016,11 @@ int fill_args(const ivid_gn_act_desc* d, bool backward, GnArgs* a, int* ve) {
 // The channels' sums take a launch of their own over the tiles before they are added over the samples when one thread would walk over
 // more tiles than this (three microseconds of it cost as much as the launch).
 constexpr int FOLD_ABOVE = 48;
+// Many samples (tokens, mostly) are added in up to 64 rows of at least 256 of them.
+int param_rows(int N) { return N <= 512 ? 1 : (N / 256 < 64 ? N / 256 : 64); }
 
-// scratch: the clusters' words, (K > MAX_K) their totals, then (backward) part [N][krows][C] and, if folded, part [N][C]
-struct Scratch { long long words, totals, part, folded, total; };
+// scratch: the clusters' words, (K > MAX_K) their totals, then (backward) part [N][krows][C], if folded part [N][C], if in rows [2][rows][C]
+struct Scratch { long long words, totals, part, folded, rows, total; };
 Scratch layout(const ivid_gn_act_desc* d, const GnArgs& a, bool backward) {
   Scratch s{};
   const Cut& q = a.cut;
@@ -1010,7 +1030,8 @@ Scratch layout(const ivid_gn_act_desc* d, const GnArgs& a, bool backward) {
     s.part = (long long)d->N * q.krows * a.C * 8;
     if (q.krows > 1 && (long long)q.krows * ((d->N + 15) / 16) > FOLD_ABOVE) s.folded = (long long)d->N * a.C * 8;
   }
-  s.total = s.words + s.totals + s.part + s.folded;
+  if (backward && param_rows(d->N) > 1) s.rows = (long long)param_rows(d->N) * a.C * 8;
+  s.total = s.words + s.totals + s.part + s.folded + s.rows;
   return s;
 }
 
@@ -1158,10 +1179,16 @@ extern "C" int ivid_gn_act_backward(const ivid_gn_act_desc* d, const float* stat
     part = folded;
     krows = 1;
   }
-#define PARAM(T)                                                                                                                    \
-  hipLaunchKernelGGL(gn_act_param_kernel<T>, dim3((unsigned)((a.C + 15) / 16)), dim3(NT_AUX), 0, st, a, (const float2*)part, krows, \
-                     d->N, dgamma, dbeta, (char*)dfilm)
+  const int rows = param_rows(d->N), per = (d->N + rows - 1) / rows;
+  float* g = s.rows ? (float*)((char*)scratch + s.total - s.rows) : dgamma;
+  float* b = s.rows ? g + (size_t)rows * a.C : dbeta;
+#define PARAM(T)                                                                                                                  \
+  hipLaunchKernelGGL(gn_act_param_kernel<T>, dim3((unsigned)((a.C + 15) / 16), (unsigned)rows), dim3(NT_AUX), 0, st, a,           \
+                     (const float2*)part, krows, d->N, per, g, b, (char*)dfilm)
   if (d->dtype == IVID_F32) PARAM(float); else if (d->dtype == IVID_BF16) PARAM(__bf16); else PARAM(_Float16);
 #undef PARAM
+  if (s.rows)
+    hipLaunchKernelGGL(gn_act_rows_kernel, dim3((unsigned)((a.C + NT_AUX - 1) / NT_AUX)), dim3(NT_AUX), 0, st, (const float*)g, (const float*)b, rows, a.C,
+                       dgamma, dbeta);
   return ivid_check_launch("gn_act_backward");
 }

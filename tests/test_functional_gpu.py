@@ -70,6 +70,8 @@ GN_CASES = [
     ("ragged_131x127_c48", (1, 131, 127), 48, 0, 8, None, "silu", 0.1),
     ("p_one", (2, 4, 4), 32, 0, 8, "f32", "silu", 1.0),
     ("many_samples", (300, 2, 2), 32, 0, 8, "f32", "silu", 0.1),
+    ("tokens_2d", (5000,), 96, 0, 8, None, "silu", 0.1),
+    ("tokens_odd_count", (1037, 1), 40, 24, 4, "same", "none", 0.0),
 ]
 
 
