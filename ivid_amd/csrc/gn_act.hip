@@ -81,6 +81,10 @@ __device__ __forceinline__ int fresh_thread() {
   return t;
 }
 
+// Every load has come back (s_waitcnt vmcnt(0)).  Behind the conditions around its pieces the compiler cannot know, and would wait for
+// "all but the last few" memory operations in front of each piece -- which by then are the results' own stores, of the same counter.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
 // f(0), f(1), ... f(N - 1) as straight-line code: the sweeps of a tile live in registers, which cannot be indexed by a loop.  No branch
 // around them either: the loads have to be unconditional for the compiler to wait for one after the other.
 template <typename F, int... I>
@@ -512,6 +516,7 @@ __global__ __launch_bounds__(NT, 4) void gn_act_fwd_kernel(GnArgs a, char* __res
   __syncthreads();
   if (t.mine <= 0) return;
   // ---- the result ----
+  loads_done();
   float sc[VE], bb[VE];
   read_channels<VE>(chM, t.piece, m);
   read_channels<VE>(chS, t.piece, sc);
@@ -770,35 +775,38 @@ __global__ __launch_bounds__(NT, 2) void gn_act_bwd_kernel(GnArgs a, const float
     gm2[g] /= Mf;
   }
   __syncthreads();
+  // dx = gv * (rstd * gamma * (1 + s)) - rstd * sum(g) / M - xc * (rstd^2 * sum(g * xhat) / M); one value a group has no gradient, which
+  // three rounded coefficients would miss by a rounding of terms that are 1 / sqrt(eps) large
+  const bool alone = Mf == 1.0f;
   for (int j = threadIdx.x; j < t.ce - t.cb; j += NT) {
     const int gj = q.by_Cg.of(t.cb + j) - slab * q.GS;
-    chA[j] = gm1[gj];
-    chB[j] = gm2[gj] * grstd[gj];
-    redA[j] = grstd[gj];
+    const float rs = alone ? 0.f : grstd[gj];
+    chA[j] = gm1[gj] * rs;
+    chB[j] = gm2[gj] * rs * rs;
+    chW[j] *= rs;
   }
   __syncthreads();
   if (t.mine <= 0) return;
   // ---- the result ----
+  loads_done();
   const bool second = t.c >= a.C0;
   const long long ld = second ? a.C - a.C0 : a.C0;
   char* o = (second ? d1 : d0) + (((long long)n * a.HW + t.row0 + t.r0) * ld + (t.c - (second ? a.C0 : 0))) * (long long)sizeof(T);
   const long long ostep2 = ld * (q.RPI * (int)sizeof(T));
   int left = t.mine;
   forget(left);
-  float m[VE], gw[VE], m1[VE], m2[VE], rs[VE];
+  float m[VE], k0[VE], k1[VE], k2[VE];
   read_channels<VE>(chM, t.piece, m);
-  read_channels<VE>(chW, t.piece, gw);
-  read_channels<VE>(chA, t.piece, m1);
-  read_channels<VE>(chB, t.piece, m2);
-  read_channels<VE>(redA, t.piece, rs);
+  read_channels<VE>(chW, t.piece, k0);
+  read_channels<VE>(chA, t.piece, k1);
+  read_channels<VE>(chB, t.piece, k2);
   sweeps<NV>([&](auto i) __attribute__((always_inline)) {
     if (left > 0) {
       float f[VE];
       forget(x[i]);
       unpack<T, VE>(x[i], f);
-      // (g is rounded before sum(g) / M is taken off: with one value a group they cancel exactly)
 #pragma unroll
-      for (int e = 0; e < VE; ++e) f[e] = rs[e] * __builtin_fmaf(m[e] - f[e], m2[e], gv[i][e] * gw[e] - m1[e]);
+      for (int e = 0; e < VE; ++e) f[e] = __builtin_fmaf(gv[i][e], k0[e], __builtin_fmaf(m[e] - f[e], k2[e], -k1[e]));
       __builtin_nontemporal_store(pack<T, VE>(f), (mem_t*)o);
     }
     o += ostep2;

@@ -130,7 +130,8 @@ def check(got, want, bound, what=""):
         g = got[k].detach().double().cpu()
         assert g.shape == ref.shape, (what, k, g.shape, ref.shape)
         assert torch.isfinite(g).all(), (what, k, "not finite")
-        r = ((g - ref).abs() / bound[k]).max().item() if ref.numel() else 0.0
+        off = (g - ref).abs()
+        r = torch.where(off == 0, 0.0, off / bound[k]).max().item() if ref.numel() else 0.0      # (0 / 0 where a bound is 0)
         assert r <= 1.0, f"{what}: {k} is {r:.3f} times its bound off"
         worst = max(worst, r)
     return worst

@@ -113,3 +113,23 @@ def test_reference_gradients_are_autograds():
     assert torch.allclose(out["y"], y.detach(), atol=1e-12)
     for k, gr in zip(("dx", "dskip", "dweight", "dbias", "dfilm"), grads):
         assert torch.allclose(out[k], gr, atol=1e-11), k
+
+
+def test_ctypes_descriptor_matches_the_header(tmp_path):
+    """sizeof and the offsets of every field, as the C compiler lays them out."""
+    import os
+    import shutil
+    import subprocess
+    import common as C
+    from ivid_amd import _lib
+    if shutil.which("gcc") is None:
+        pytest.skip("no C compiler")
+    names = [n for n, _ in _lib.GnActDesc._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "ivid_hip.h"\nint main(void) {\n'
+                   + "".join(f'  printf("%zu\\n", offsetof(ivid_gn_act_desc, {n}));\n' for n in names)
+                   + '  printf("%zu\\n", sizeof(ivid_gn_act_desc));\n  return 0;\n}\n')
+    exe = tmp_path / "layout"
+    subprocess.check_call(["gcc", "-I" + os.path.join(C.ROOT, "include"), str(src), "-o", str(exe)])
+    got = [int(v) for v in subprocess.check_output([str(exe)]).split()]
+    assert got == [getattr(_lib.GnActDesc, n).offset for n in names] + [ctypes.sizeof(_lib.GnActDesc)]

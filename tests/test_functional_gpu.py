@@ -476,3 +476,80 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(dx[2:], dx1)
     del x, y, dx, dx1
     torch.cuda.empty_cache()
+
+
+def test_backward_twice_and_one_tensor_in_two_places():
+    t = gn_inputs(121, (2, 9, 9), 48, 0, torch.float32, "f32")
+    x, w = t["x"].requires_grad_(), (1 + 0.1 * randn(1, 96)).requires_grad_()
+    b = randn(2, 96) * 0.1
+    film = (0.3 * randn(3, 1, 192)).requires_grad_()
+    dy = randn(4, 2, 9, 9, 96)
+    rng = torch.tensor([3, 4], device="cuda")
+    y = F().group_norm_act(x, 12, w, b, film=film.expand(2, 192), skip=x, p=0.1, rng=rng)
+    a = torch.autograd.grad(y, [x, w, film], dy, retain_graph=True)
+    c = torch.autograd.grad(y, [x, w, film], dy)
+    for p, q in zip(a, c):
+        assert torch.equal(p, q)
+    want, bound = R.gn_act(x, 12, w, b, film=film.expand(2, 192), skip=x, dy=dy, p=0.1, rng=(3, 4))
+    got = dict(y=y, dx=a[0], dweight=a[1], dfilm=a[2])
+    for k, both in (("dx", "dskip"), ("dfilm", None)):
+        if both:
+            want[k], bound[k] = want[k] + want[both], bound[k] + bound[both] + R.U * (want[k].abs() + want[both].abs())
+        else:
+            want[k], bound[k] = want[k].sum(0, keepdim=True), bound[k].sum(0, keepdim=True) + 2 * R.U * want[k].abs().sum(0, keepdim=True)
+    R.check(got, {k: want[k] for k in got}, bound)
+
+
+def test_saved_tensors_may_be_moved_or_recomputed():
+    from torch.utils.checkpoint import checkpoint
+    t = gn_inputs(131, (3, 20, 20), 64, 0, torch.bfloat16, "f32")
+    x, w, b, film = t["x"].requires_grad_(), t["weight"].requires_grad_(), t["bias"].requires_grad_(), t["film"].requires_grad_()
+    dy = randn(5, 3, 20, 20, 64, dtype=torch.bfloat16)
+
+    def block(x, w, b, film):
+        return F().dropout(F().group_norm_act(x, 8, w, b, film=film, p=0.1, rng=RNG), 0.2, (9, 9))
+    ref = torch.autograd.grad(block(x, w, b, film), [x, w, b, film], dy)
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: s.cpu(), lambda s: s.cuda()):
+        y = block(x, w, b, film)
+    for p, q in zip(ref, torch.autograd.grad(y, [x, w, b, film], dy)):
+        assert torch.equal(p, q)
+    y = checkpoint(block, x, w, b, film, use_reentrant=False)
+    for p, q in zip(ref, torch.autograd.grad(y, [x, w, b, film], dy)):
+        assert torch.equal(p, q)
+
+
+def test_a_constant_sample():
+    """No variance: xhat is 0 to the rounding of the mean, rstd 1 / sqrt(eps) -- 10^4 with eps = 10^-8 --, and nothing is NaN."""
+    x = torch.full((2, 17, 64), 3.0, device="cuda")
+    x[1] = 0
+    w, b = torch.ones(64, device="cuda"), randn(1, 64)
+    for eps in (1e-5, 1e-8):
+        want, bound = R.gn_act(x, 8, w, b, eps=eps)
+        y, stats = F().group_norm_act_forward(x, 8, w, b, eps=eps)
+        R.check(dict(y=y, stats=stats), want, bound)
+        assert torch.isfinite(y).all()
+    dx = F().group_norm_act_backward(randn(2, 2, 17, 64), stats, x, 8, w, b, eps=1e-8)[0]
+    assert torch.isfinite(dx).all()
+
+
+def test_python_entry_points_refuse_what_does_not_fit():
+    f = F()
+    x, w, b = randn(1, 2, 4, 32), torch.ones(32, device="cuda"), torch.zeros(32, device="cuda")
+    bad = [(ValueError, dict(groups=5)), (ValueError, dict(groups=0)), (TypeError, dict(weight=w.half())), (ValueError, dict(weight=w[:16])),
+           (ValueError, dict(bias=b.cpu())), (ValueError, dict(film=randn(1, 2, 32))), (TypeError, dict(film=randn(1, 2, 64).double())),
+           (ValueError, dict(film=randn(1, 3, 64))), (ValueError, dict(skip=randn(1, 2, 5, 32))), (ValueError, dict(skip=randn(1, 2, 4, 8).half())),
+           (ValueError, dict(skip=randn(1, 2, 4, 0))), (ValueError, dict(act="gelu")), (ValueError, dict(eps=0.0)),
+           (ValueError, dict(eps=float("inf"))), (ValueError, dict(p=1.5, rng=RNG)), (ValueError, dict(p=0.5)),
+           (ValueError, dict(p=0.5, rng=torch.zeros(2, dtype=torch.int32, device="cuda"))),
+           (ValueError, dict(p=0.5, rng=torch.zeros(2, dtype=torch.int64))), (TypeError, dict(x=x.double())), (ValueError, dict(x=randn(1, 32)))]
+    for err, kw in bad:
+        args = dict(dict(x=x, groups=8, weight=w, bias=b), **kw)
+        with pytest.raises(err):
+            f.group_norm_act(**args)
+    y, stats = f.group_norm_act_forward(x, 8, w, b)
+    for dy, st in ((y[:1], stats), (y.half(), stats), (y, stats[:1]), (y, stats.double()), (y.cpu(), stats)):
+        with pytest.raises(ValueError):
+            f.group_norm_act_backward(dy, st, x, 8, w, b)
+    dy = torch.empty(2 * 4 * 32 + 1, device="cuda")[1:].view(2, 4, 32).copy_(y)      # a gradient that is not on 16 bytes
+    for p, q in zip(f.group_norm_act_backward(dy, stats, x, 8, w, b), f.group_norm_act_backward(y, stats, x, 8, w, b)):
+        assert (p is None and q is None) or torch.equal(p, q)
