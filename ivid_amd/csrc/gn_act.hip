@@ -325,48 +325,61 @@ __device__ __forceinline__ void add_runs(const Cut& q, float* v) {
     if (q.seg >= 8) v[0] += v[4];
   }
 }
-// Sum over the tile of one value a channel and thread, per group: gs[g] (LDS), the same order for every workgroup.  A run is one word in
-// LDS; a team of W lanes adds its group's.
-template <int VE>
-__device__ __forceinline__ void group_sums(const GnArgs& a, const Tile& t, int slab, float* v, float* red, float* gs) {
+// Sums over the tile of M values a channel and thread, per group: gs[m][g] (LDS), the same order for every workgroup.  A run is one word
+// in LDS (red[m], NT * VE of them); a team of W lanes adds its group's.
+template <int VE, int M>
+__device__ __forceinline__ void group_sums(const GnArgs& a, const Tile& t, int slab, float (&v)[M][VE], float* const (&red)[M], float* const (&gs)[M]) {
   const Cut& q = a.cut;
   const int thread = fresh_thread();
-  add_runs<VE>(q, v);
+#pragma unroll
+  for (int k = 0; k < M; ++k) add_runs<VE>(q, v[k]);
   const int RS = q.PP * (VE >> q.logseg);      // runs of a row
   if (thread < q.RPI * q.PP) {
     const int first = (thread * VE) >> q.logseg;      // a thread's runs follow those of the thread in front
 #pragma unroll
     for (int e = 0; e < VE; ++e)
-      if ((e & (q.seg - 1)) == 0) red[first + (e >> q.logseg)] = v[e];
+      if ((e & (q.seg - 1)) == 0) {
+#pragma unroll
+        for (int k = 0; k < M; ++k) red[k][first + (e >> q.logseg)] = v[k][e];
+      }
   }
   __syncthreads();
   const int g = thread >> q.logW, W = 1 << q.logW, l = thread & (W - 1);
   const int c0 = slab * q.S + g * a.Cg;
   const int lo = (max(c0, t.cb) - t.cb) >> q.logseg, hi = g < groups_of(a, slab) ? (min(c0 + a.Cg, t.ce) - t.cb) >> q.logseg : 0;
   const int w = max(hi - lo, 0), rows = min(q.RPI, t.nrow);
-  float sum = 0.f;
+  float sum[M];
+#pragma unroll
+  for (int k = 0; k < M; ++k) sum[k] = 0.f;
   if (w > 0) {
     const bool whole = w == a.Cg >> q.logseg;
     const int dr = whole ? q.by_runs.of(W) : W / w, dj = W - dr * w;
     int row = whole ? q.by_runs.of(l) : l / w;
     int j = l - row * w;
     while (row < rows) {
-      sum += red[row * RS + lo + j];
+#pragma unroll
+      for (int k = 0; k < M; ++k) sum[k] += red[k][row * RS + lo + j];
       row += dr;
       j += dj;
       if (j >= w) { j -= w; ++row; }
     }
   }
-  for (int o = W >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-  if (l == 0 && g < q.GS) gs[g] = sum;
+  for (int o = W >> 1; o > 0; o >>= 1) {
+#pragma unroll
+    for (int k = 0; k < M; ++k) sum[k] += __shfl_xor(sum[k], o);
+  }
+  if (l == 0 && g < q.GS) {
+#pragma unroll
+    for (int k = 0; k < M; ++k) gs[k][g] = sum[k];
+  }
   __syncthreads();
 }
 
 // A thread's channel sums s[] -> the means of the tile's groups in gmean[] (LDS) and, of each of the thread's channels, in m[].
 template <int VE>
-__device__ __forceinline__ void tile_means(const GnArgs& a, const Tile& t, int slab, float* s, float* m, float* red, float* gmean) {
+__device__ __forceinline__ void tile_means(const GnArgs& a, const Tile& t, int slab, float (&s)[1][VE], float* m, float* red, float* gmean) {
   const Cut& q = a.cut;
-  group_sums<VE>(a, t, slab, s, red, gmean);
+  group_sums<VE, 1>(a, t, slab, s, {red}, {gmean});
   const int g = fresh_thread();
   if (g < groups_of(a, slab)) gmean[g] /= fmaxf((float)t.nrow * (float)columns_of(a, slab, t.kc, g, VE), 1.f);
   __syncthreads();
@@ -385,11 +398,11 @@ __device__ __forceinline__ void tile_means(const GnArgs& a, const Tile& t, int s
 template <typename T, int VE>
 __device__ __forceinline__ void help_forward(const GnArgs& a, int n, int slab, int k, float* red, float* gmean, float* gsq) {
   const Tile t = tile_of<VE>(a, slab, k, fresh_thread());
-  float s[VE], m[VE];
+  float s[1][VE], m[VE];
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
-    for (int e = 0; e < VE; ++e) s[e] = 0.f;
+    for (int e = 0; e < VE; ++e) s[0][e] = 0.f;
     Source<T, VE> src(a, n, t);
 #pragma unroll 1
     for (int left = t.mine; left > 0; left -= a.cut.RPI) {
@@ -397,14 +410,14 @@ __device__ __forceinline__ void help_forward(const GnArgs& a, int n, int slab, i
       unpack<T, VE>(*(const typename Piece<T, VE>::mem*)src.p, f);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        if (pass == 0) s[e] += f[e];
-        else { const float d = f[e] - m[e]; s[e] = __builtin_fmaf(d, d, s[e]); }
+        if (pass == 0) s[0][e] += f[e];
+        else { const float d = f[e] - m[e]; s[0][e] = __builtin_fmaf(d, d, s[0][e]); }
       }
       src.p += src.step;
     }
     if (pass == 0) tile_means<VE>(a, t, slab, s, m, red, gmean);
   }
-  group_sums<VE>(a, t, slab, s, red, gsq);
+  group_sums<VE, 1>(a, t, slab, s, {red}, {gsq});
 }
 
 template <int NT, typename T, int VE, int NV>
@@ -442,9 +455,9 @@ __global__ __launch_bounds__(NT, 4) void gn_act_fwd_kernel(GnArgs a, char* __res
     chB[j] = wb.y;
   });
   // ---- means and centred squares ----
-  float s[VE], m[VE];
+  float s[1][VE], m[VE];
 #pragma unroll
-  for (int e = 0; e < VE; ++e) s[e] = 0.f;
+  for (int e = 0; e < VE; ++e) s[0][e] = 0.f;
   {
     int left = t.mine;
     forget(left);
@@ -454,13 +467,13 @@ __global__ __launch_bounds__(NT, 4) void gn_act_fwd_kernel(GnArgs a, char* __res
         forget(x[i]);
         unpack<T, VE>(x[i], f);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) s[e] += f[e];
+        for (int e = 0; e < VE; ++e) s[0][e] += f[e];
       }
       left -= q.RPI;
     });
     tile_means<VE>(a, t, slab, s, m, red, gmean);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) s[e] = 0.f;
+    for (int e = 0; e < VE; ++e) s[0][e] = 0.f;
     left = t.mine;
     forget(left);
     sweeps<NV>([&](auto i) __attribute__((always_inline)) {
@@ -469,11 +482,11 @@ __global__ __launch_bounds__(NT, 4) void gn_act_fwd_kernel(GnArgs a, char* __res
         forget(x[i]);
         unpack<T, VE>(x[i], f);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) { const float d = f[e] - m[e]; s[e] = __builtin_fmaf(d, d, s[e]); }
+        for (int e = 0; e < VE; ++e) { const float d = f[e] - m[e]; s[0][e] = __builtin_fmaf(d, d, s[0][e]); }
       }
       left -= q.RPI;
     });
-    group_sums<VE>(a, t, slab, s, red, gsq);
+    group_sums<VE, 1>(a, t, slab, s, {red}, {gsq});
   }
   const int GS = groups_of(a, slab), g = threadIdx.x;
   if (q.K == 1) {
@@ -577,13 +590,25 @@ __device__ __forceinline__ void bwd_channels(const GnArgs& a, int n, int slab, c
   });
   __syncthreads();
 }
-// The threads' channel sums A, B (of gv and gv * xc) -> those of the tile (chA, chB; done(j, A, B) for each) and of its groups (gm1, gm2:
-// sums of g and g * xhat).
+// The threads' channel sums A, B (of gv and gv * xc) -> the sums of g and g * xhat of the tile's groups, gm1 and gm2.
+template <int VE>
+__device__ __forceinline__ void group_gradients(const GnArgs& a, const Tile& t, int slab, const float* A, const float* B, const BwdShared& h) {
+  float gw[VE], sc[VE], v[2][VE];
+  read_channels<VE>(h.chW, t.piece, gw);
+  read_channels<VE>(h.chB, t.piece, sc);
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    v[0][e] = t.mine > 0 ? A[e] * gw[e] : 0.f;
+    v[1][e] = t.mine > 0 ? B[e] * sc[e] : 0.f;
+  }
+  group_sums<VE, 2>(a, t, slab, v, {h.redA, h.redB}, {h.gm1, h.gm2});
+}
+// ... -> those of the tile's channels, of gv and gv * xhat: done(j, A, B) for each.
 template <int NT, int VE, typename F>
-__device__ __forceinline__ void join_gradients(const GnArgs& a, const Tile& t, int slab, const float* A, const float* B, const BwdShared& h, F done) {
+__device__ __forceinline__ void channel_gradients(const GnArgs& a, const Tile& t, int slab, const float* A, const float* B, const BwdShared& h, F done) {
   const Cut& q = a.cut;
   const int thread = fresh_thread();
-  const int RS = q.PP * VE + 8, ncol = t.ce - t.cb;
+  const int RS = q.PP * VE + 8, ncol = t.ce - t.cb;      // (padded: several rows are read at once)
   if (t.r0 < q.RPI) {
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
@@ -611,30 +636,8 @@ __device__ __forceinline__ void join_gradients(const GnArgs& a, const Tile& t, i
   for (int j = thread; j < ncol; j += NT) {
     float sa = 0.f, sb = 0.f;
     for (int r = 0; r < nr; ++r) { sa += h.redA[r * rs + j]; sb += h.redB[r * rs + j]; }
-    sb *= h.grstd[q.by_Cg.of(t.cb + j) - slab * q.GS];
-    h.chA[j] = sa;
-    h.chB[j] = sb;
-    done(j, sa, sb);
+    done(j, sa, sb * h.grstd[q.by_Cg.of(t.cb + j) - slab * q.GS]);
   }
-  __syncthreads();
-  const int g = thread >> q.logW, W = 1 << q.logW, l = thread & (W - 1);
-  const int c0 = slab * q.S + g * a.Cg;
-  float s1 = 0.f, s2 = 0.f;
-  if (g < groups_of(a, slab)) {
-    for (int j = max(c0, t.cb) - t.cb + l; j < min(c0 + a.Cg, t.ce) - t.cb; j += W) {
-      s1 += h.chA[j] * h.chW[j];
-      s2 += h.chB[j] * h.chW[j];
-    }
-  }
-  for (int o = W >> 1; o > 0; o >>= 1) {
-    s1 += __shfl_xor(s1, o);
-    s2 += __shfl_xor(s2, o);
-  }
-  if (l == 0 && g < q.GS) {
-    h.gm1[g] = s1;
-    h.gm2[g] = s2;
-  }
-  __syncthreads();
 }
 
 template <int NT, typename T, int VE>
@@ -661,7 +664,7 @@ __device__ __forceinline__ void help_backward(const GnArgs& a, int n, int slab, 
     src.p += src.step;
     o += (long long)a.cut.RPI * a.C;
   }
-  join_gradients<NT, VE>(a, t, slab, A, B, h, [](int, float, float) {});
+  group_gradients<VE>(a, t, slab, A, B, h);
 }
 
 template <int NT, typename T, int VE, int NV>
@@ -671,7 +674,7 @@ __global__ __launch_bounds__(NT, 2) void gn_act_bwd_kernel(GnArgs a, const float
   typedef typename Piece<T, VE>::reg reg_t;
   typedef typename Piece<T, VE>::mem mem_t;
   __shared__ __attribute__((aligned(16))) float redA[NT * (VE + 8)], redB[NT * (VE + 8)];
-  // per channel: mean, gamma * (1 + s), the offset (then A), the scale (then B)
+  // per channel: mean, gamma * (1 + s), offset and scale; afterwards the coefficients of the result
   __shared__ __attribute__((aligned(16))) float chM[MAX_COL], chW[MAX_COL], chA[MAX_COL], chB[MAX_COL];
   __shared__ float gmean[MAX_GS], grstd[MAX_GS], gm1[MAX_GS], gm2[MAX_GS];
   __shared__ double2 tot[MAX_GS];
@@ -685,6 +688,8 @@ __global__ __launch_bounds__(NT, 2) void gn_act_bwd_kernel(GnArgs a, const float
   const Tile t = tile_of<VE>(a, slab, me, threadIdx.x);
   const int GS = groups_of(a, slab), g = threadIdx.x;
   const long long o0 = ((long long)n * a.HW + t.row0 + t.r0) * a.C + t.c, ostep = (long long)q.RPI * a.C;
+
+  unsigned long long* const cluster = words + ((size_t)n * q.nslab + slab) * q.K * q.GS * 2;
 
   reg_t x[NV];
   float gv[NV][VE];
@@ -739,25 +744,30 @@ __global__ __launch_bounds__(NT, 2) void gn_act_bwd_kernel(GnArgs a, const float
       o += ostep;
       left -= q.RPI;
     });
-    join_gradients<NT, VE>(a, t, slab, A, B, h, [&](int j, float sa, float sb) __attribute__((always_inline)) {
+    // the groups' sums go out first: the others wait for them while the channels' are added
+    group_gradients<VE>(a, t, slab, A, B, h);
+    if (q.K > 1 && q.phase != PH_RESULT && g < GS) {
+      publish(cluster + ((size_t)me * q.GS + g) * 2, gm1[g]);
+      publish(cluster + ((size_t)me * q.GS + g) * 2 + 1, gm2[g]);
+    }
+    channel_gradients<NT, VE>(a, t, slab, A, B, h, [&](int j, float sa, float sb) __attribute__((always_inline)) {
       part[((size_t)n * q.krows + (q.kcols > 1 ? me / q.kcols : me)) * a.C + t.cb + j] = make_float2(sa, sb);
     });
   }
+  if (q.phase == PH_SUMS) return;
   const float Mf = (float)a.HW * (float)a.Cg;
   if (q.K > 1) {
     bool helped = false;
     if (q.phase != PH_RESULT) {
-      unsigned long long* const cluster = words + ((size_t)n * q.nslab + slab) * q.K * q.GS * 2;
-      for (int k = me;;) {
+      for (;;) {
+        const int k = gather<VE, false>(a, slab, cluster, &missing, tot);
+        if (k < 0) break;
+        help_backward<NT, T, VE>(a, n, slab, k, dy, h);
+        helped = true;
         if (g < GS) {
           publish(cluster + ((size_t)k * q.GS + g) * 2, gm1[g]);
           publish(cluster + ((size_t)k * q.GS + g) * 2 + 1, gm2[g]);
         }
-        if (q.phase == PH_SUMS) return;
-        k = gather<VE, false>(a, slab, cluster, &missing, tot);
-        if (k < 0) break;
-        help_backward<NT, T, VE>(a, n, slab, k, dy, h);
-        helped = true;
       }
     }
     if (g < GS) {
