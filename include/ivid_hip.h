@@ -286,7 +286,7 @@ int ivid_gn_apply_p(int dtype, const void* src0, const void* src0_lo, int C0, co
  * x = cat[src0, src1] over channels, N samples of HW pixels; mean and biased variance per (sample, group) in fp32 or wider;
  * act 0 none, 1 SiLU; drop as in ivid_dropout, element index = row-major index in the [N,HW,C0+C1] output.
  * Any N, HW >= 1, any C0 + C1 divisible by groups; src0, src1, gamma, beta and film may be aligned to an element only, every other
- * pointer of a tensor to 16 bytes. */
+ * pointer of a tensor to 16 bytes.  Outputs and scratch overlap neither the inputs nor each other (not even in place). */
 typedef struct {
   int dtype;                              /* IVID_F32, IVID_BF16 or IVID_F16: src, out, dy, dsrc */
   int N, HW, C0, C1, groups, act;         /* C1 = 0 and src1 = NULL: one source */
@@ -405,7 +405,7 @@ int ivid_randn(unsigned long long seed, unsigned long long stream_id, float* out
  * every p < 1 (p is used in steps of 2^-16); p = 1 drops all.  draw(i) = 16 bits, half i % 2 (low first) of word (i % 8) / 2 of the
  * Philox4x32-10 block with counter (i / 8, stream_id) and key seed ^ 0x44524F50 << 32: a pure function of (seed, stream_id, i), so the
  * backward pass is the same call on the gradient, and independent of ivid_randn's values for the same (seed, stream_id).
- * A dropped element is 0 whatever x holds.  x == out is allowed.  rng: NULL, or device {seed, stream_id} read when the kernel runs
+ * A dropped element is 0 whatever x holds.  x == out is allowed, another overlap is not.  rng: NULL, or device {seed, stream_id} read when the kernel runs
  * instead of the arguments (a captured graph then draws anew when the host rewrites them between replays). */
 int ivid_dropout(int dtype, const void* x, void* out, long long n, double p, unsigned long long seed, unsigned long long stream_id,
                  const unsigned long long* rng, void* stream);

@@ -1,7 +1,8 @@
 // Dropout from the counter-based generator (philox.h): the draws are a function of (seed, stream, element index), so no mask is
 // stored and the backward pass is the same kernel on the gradient.
 //
-// A thread takes whole generator blocks of eight elements, STEPS of them, all loads in front of the generator's rounds.
+// A thread takes whole generator blocks of eight elements, STEPS of them, all loads in front of the generator's rounds: bound by HBM,
+// 188 us for 64 x 128 x 128 x 256 bf16 (537 MB in, 537 MB out: 5.7 TB/s; a copy 202 us), where one element a thread ran 558.
 #include <math.h>
 #include "common.h"
 #include "internal.h"
@@ -88,6 +89,9 @@ extern "C" int ivid_dropout(int dtype, const void* x, void* out, long long n, do
   if (n == 0) return 0;
   if (!x || !out || (((uintptr_t)x | (uintptr_t)out) % esz) || ((uintptr_t)rng & 7))
     return ivid_set_error("dropout: NULL or misaligned pointer", hipSuccess);
+  const uintptr_t px = (uintptr_t)x, po = (uintptr_t)out;
+  if (px != po && (px < po ? po - px : px - po) / esz < (unsigned long long)n)
+    return ivid_set_error("dropout: x and out overlap and are not the same", hipSuccess);
   hipStream_t s = (hipStream_t)stream;
   if (dtype == IVID_F32) return launch<float>(x, out, n, r, s);
   return dtype == IVID_F16 ? launch<_Float16>(x, out, n, r, s) : launch<__bf16>(x, out, n, r, s);

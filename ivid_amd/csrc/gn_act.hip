@@ -17,6 +17,21 @@
 // A cluster of more than MAX_K tiles would not be resident at once: it takes two launches, sums and results (PH_SUMS, PH_RESULT), with
 // a small one between them that adds the words, and reads its inputs twice.
 // Squares are centred on the tile's own means: a large mean costs no digits.
+//
+// Choices and what they measured (MI355X; 64 x 128 x 128 x 256 bf16; copying that tensor takes 202 us, 5.3 TB/s).  A variant's
+// time stands next to that of the form it was compared with, on the same card: several steps lie between some of them.
+//   * now: forward 238 us (4.5 TB/s; with dropout 272), backward 374 (4.3 TB/s; 421).  One workgroup per (sample, group) with three
+//     passes over memory: forward 2793, a training step with dropout 15699 (now 690);
+//   * forward: 512 threads x 16 pieces (128 KB of x a workgroup) 293; 256 threads x 16 pieces 298, 1024 x 16: 322, 512 x 8: 323.
+//     Backward: 256 threads x 12 pieces, x and the fp32 gradient behind the activation kept, 464; 512 threads 582; 10 pieces 522,
+//     16: 527;
+//   * a cluster's workgroups next to each other in the grid: forward 337 -> 309, backward 571 -> 506;
+//   * loads without branches around them and coefficients in front of the tile, so that the compiler waits for one piece after the
+//     other while the sums run, with lighter joins: forward 317 -> 255, backward 570 -> 433;
+//   * the group sums published in front of the channel sums: backward 425 -> 374;
+//   * slabs of 64 bytes 255 / 488 where 128 ran 238 / 426; of 256 bytes 302 / 528 where 128 ran 309 / 506 (forward / backward);
+//   * what is left: the vector units are busy 64 % (forward) and 59 % (backward) of the time by the counters, and a workgroup reads, sums,
+//     waits and writes in turn, so that these overlap with memory between workgroups only.
 #include <math.h>
 #include <utility>
 #include "common.h"
@@ -1018,7 +1033,7 @@ int fill_args(const ivid_gn_act_desc* d, bool backward, GnArgs* a, int* ve) {
   if ((d->C1 > 0) != (d->src1 != nullptr)) return ivid_set_error("gn_act: src1 and C1 go together", hipSuccess);
   if (d->ld0 < 0 || d->sn0 < 0 || d->ld1 < 0 || d->sn1 < 0 || d->film_ld < 0) return ivid_set_error("gn_act: negative stride", hipSuccess);
   if (d->act != 0 && d->act != 1) return ivid_set_error("gn_act: bad act", hipSuccess);
-  if (!(d->eps > 0.0)) return ivid_set_error("gn_act: eps must be positive", hipSuccess);
+  if (!((float)d->eps > 0.0f && d->eps <= 3.4e38)) return ivid_set_error("gn_act: eps must be positive and finite in fp32", hipSuccess);
   if (d->film && d->film_dtype != IVID_F32 && d->film_dtype != d->dtype) return ivid_set_error("gn_act: film must be fp32 or of the tensors' dtype", hipSuccess);
   if (!d->src0 || !d->gamma || !d->beta || ((uintptr_t)d->src0 | (uintptr_t)d->src1) % esz || ((uintptr_t)d->gamma | (uintptr_t)d->beta) % 4 ||
       (uintptr_t)d->film % (d->film_dtype == IVID_F32 ? 4 : esz) || (uintptr_t)d->rng % 8)
@@ -1061,6 +1076,20 @@ int clear_words(const Scratch& s, void* scratch, hipStream_t stream) {
   return 0;
 }
 
+// A workgroup that helps reads another one's inputs when that may already have written results: no output may lie over an input.
+// p: `bytes` contiguous ones.  (128 bits: strides are the caller's.)
+bool meets(const void* p, __int128 bytes, const void* q, __int128 qbytes) {
+  const __int128 a = (uintptr_t)p, b = (uintptr_t)q;
+  return p && q && a < b + qbytes && b < a + bytes;
+}
+__int128 source_bytes(const ivid_gn_act_desc* d, bool second) {
+  const long long ld = second ? d->ld1 : d->ld0, sn = second ? d->sn1 : d->sn0;
+  return ((__int128)(d->N - 1) * sn + (__int128)(d->HW - 1) * ld + (second ? d->C1 : d->C0)) * ivid_esz(d->dtype);
+}
+bool meets_sources(const ivid_gn_act_desc* d, const void* p, __int128 bytes) {
+  return meets(p, bytes, d->src0, source_bytes(d, false)) || meets(p, bytes, d->src1, source_bytes(d, true));
+}
+
 // `run` launches the kernel once, or as sums - totals - results
 template <int NT, bool MOMENTS, typename Run>
 void run_phases(GnArgs& a, const ivid_gn_act_desc* d, int ve, const Scratch& s, void* scratch, hipStream_t st, Run run) {
@@ -1092,6 +1121,7 @@ extern "C" int ivid_gn_act_forward(const ivid_gn_act_desc* d, void* out, float* 
   int ve;
   if (int e = fill_args(d, false, &a, &ve)) return e;
   if (!out || !stats || ((uintptr_t)out & 15) || ((uintptr_t)stats & 3)) return ivid_set_error("gn_act: out / stats missing or misaligned", hipSuccess);
+  if (meets_sources(d, out, (__int128)d->N * d->HW * a.C * ivid_esz(d->dtype))) return ivid_set_error("gn_act_forward: out overlaps a source", hipSuccess);
   const Scratch s = layout(d, a, false);
   if (scratch_bytes < s.total || (s.total && (!scratch || ((uintptr_t)scratch & 15)))) return ivid_set_error("gn_act: scratch too small or misaligned", hipSuccess);
   hipStream_t st = (hipStream_t)stream;
@@ -1147,6 +1177,10 @@ extern "C" int ivid_gn_act_backward(const ivid_gn_act_desc* d, const float* stat
   if (!stats || !dy || !dsrc0 || (((uintptr_t)dy | (uintptr_t)dsrc0 | (uintptr_t)dsrc1) & 15) ||
       ((uintptr_t)stats & 7) || (((uintptr_t)dgamma | (uintptr_t)dbeta | (uintptr_t)dfilm) & 3))
     return ivid_set_error("gn_act_backward: NULL or misaligned pointer", hipSuccess);
+  const __int128 pixels = (__int128)d->N * d->HW * ivid_esz(d->dtype);
+  if (meets_sources(d, dsrc0, pixels * d->C0) || meets_sources(d, dsrc1, pixels * d->C1) || meets(dsrc0, pixels * d->C0, dy, pixels * a.C) ||
+      meets(dsrc1, pixels * d->C1, dy, pixels * a.C) || meets(dsrc0, pixels * d->C0, dsrc1, pixels * d->C1))
+    return ivid_set_error("gn_act_backward: dsrc0 or dsrc1 overlaps another tensor", hipSuccess);
   const Scratch s = layout(d, a, true);
   if (scratch_bytes < s.total || !scratch || ((uintptr_t)scratch & 15)) return ivid_set_error("gn_act_backward: scratch too small or misaligned", hipSuccess);
   hipStream_t st = (hipStream_t)stream;

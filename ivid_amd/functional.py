@@ -13,8 +13,9 @@ kernels run, so that a captured graph draws anew once the host has rewritten it;
 the forward's values (autograd's version check refuses a rewrite in between in eager code).
 
 Capturing a training step into a graph: use the `*_forward` / `*_backward` pairs, which launch kernels and nothing else.  Under
-capture the autograd forms are refused for leaves that require gradients, because accumulating into a leaf whose earlier eager
-graph still lives would make the capturing stream wait for that graph's stream, which ends the process.
+capture the operators refuse tensors that require gradients, leaves or not, because accumulating into a leaf whose earlier eager
+graph still lives would make the capturing stream wait for that graph's stream, which ends the process.  For the same reason do
+not capture the backward pass of a graph that was built in eager code.
 """
 import ctypes as C
 import math
@@ -26,6 +27,7 @@ from . import _lib
 
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _ACTS = {"none": 0, "silu": 1}
+_INT_MAX = (1 << 31) - 1
 _MAX_POLLS = 0      # ivid_gn_act_desc.max_polls; the tests lower it
 
 
@@ -77,9 +79,9 @@ def _launch(name, device, *args):
         _lib.check(status, name)
 
 
-def _refuse_captured_leaves(*tensors):
-    if torch.cuda.is_current_stream_capturing() and any(t is not None and t.requires_grad and t.is_leaf for t in tensors):
-        raise _lib.IvidHipError("autograd through a leaf under graph capture: use the *_forward / *_backward functions "
+def _refuse_capture():
+    if torch.cuda.is_current_stream_capturing():
+        raise _lib.IvidHipError("autograd under graph capture: use the *_forward / *_backward functions, or no_grad "
                                 "(see ivid_amd.functional)")
 
 
@@ -128,7 +130,7 @@ def dropout(x, p, rng=None):
     _check_x(x, "x")
     p = _check_p(p)
     if torch.is_grad_enabled() and x.requires_grad:
-        _refuse_captured_leaves(x)
+        _refuse_capture()
         return _Dropout.apply(x, p, rng)
     return _dropout(x, p, rng)
 
@@ -191,19 +193,22 @@ class _Call:
             raise ValueError(f"eps must be positive, got {eps}")
         p = _check_p(p)
         numel = x.numel()
+        hw = numel // (n * c0) if numel else 0
+        if max(n, hw, c) > _INT_MAX:      # the descriptor's ints would wrap without a word
+            raise ValueError(f"[{n}, {hw}, {c}] is too large: every size must be below 2^31")
         self.device, self.dtype = dev, dtype
         self.film_dtype = film.dtype if film is not None else None
         self.shape = shape if c1 == 0 else shape[:-1] + (c,)
         self.n, self.c0, self.c1, self.c, self.groups, self.p = n, c0, c1, c, groups, p
         self.empty = numel == 0
-        self.backward_bytes = None
-        d = self.desc = _lib.GnActDesc(_DTYPES[dtype], n, 0 if self.empty else numel // (n * c0), c0, c1, groups, _ACTS[act])
+        d = self.desc = _lib.GnActDesc(_DTYPES[dtype], n, hw, c0, c1, groups, _ACTS[act])
         d.eps, d.p, d.max_polls = eps, p, _MAX_POLLS
         self.bind(x, weight, bias, film, skip, rng)
 
     def bind(self, x, weight, bias, film, skip, rng):
         """Point the descriptor at these tensors (of the shapes and types checked in front), which the caller keeps alive."""
         d = self.desc
+        self.backward_bytes = None      # depends on strides and alignment
         self.strides = (x.stride(), weight.stride(), bias.stride(), None if film is None else film.stride(),
                         None if skip is None else skip.stride())
         self.in_place = (x.is_contiguous() and weight.is_contiguous() and bias.is_contiguous()
@@ -226,11 +231,14 @@ class _Call:
         if self.in_place and self.strides == (x.stride(), weight.stride(), bias.stride(), None if film is None else film.stride(),
                                               None if skip is None else skip.stride()):
             d = self.desc
+            before = d.src0, d.src1
             d.src0, d.gamma, d.beta = x.data_ptr(), weight.data_ptr(), bias.data_ptr()
             if film is not None:
                 d.film = film.data_ptr()
             if skip is not None:
                 d.src1 = skip.data_ptr()
+            if before != (d.src0, d.src1):
+                self.backward_bytes = None
             if d.rng:
                 d.rng = rng.data_ptr()
         else:
@@ -346,7 +354,7 @@ def group_norm_act(x, groups, weight, bias, film=None, skip=None, act="silu", ep
     Returns [N, ..., C] of x's type; statistics, sums and the arithmetic are 32 bits or wider whatever x's type, the result is rounded
     once.  Differentiable once in x, skip, weight, bias and film."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, film, skip)):
-        _refuse_captured_leaves(x, weight, bias, film, skip)
+        _refuse_capture()
         return _GroupNormAct.apply(x, weight, bias, film, skip, groups, act, eps, p, rng)
     return _Call(x, groups, weight, bias, film, skip, act, eps, p, rng).forward()[0]
 

@@ -91,6 +91,46 @@ def test_dropout_entry_point_refuses_bad_arguments():
     assert lib.ivid_dropout(0, None, None, 0, 0.5, 1, 2, None, None) == 0
 
 
+def test_eps_that_fp32_does_not_hold_is_refused():
+    from ivid_amd import _lib
+    lib = _lib.load()
+    for eps in (1e-50, 1e39, float("inf"), -1e-5):
+        d, _ = _desc(eps=eps)
+        assert lib.ivid_gn_act_scratch_bytes(ctypes.byref(d), 0) == -1, eps
+
+
+def _address(k):
+    """16-byte aligned addresses that are never read: every call here is refused on the host"""
+    return (1 << 24) + k
+
+
+def test_overlapping_tensors_are_refused():
+    from ivid_amd import _lib
+    lib = _lib.load()
+    msg = lambda: lib.ivid_last_error().decode()
+    # one sample of 4 pixels x 8 channels fp32 (128 bytes), a second source of 8 channels behind it with pixels 16 floats apart
+    ptr = dict(gamma=_address(1 << 16), beta=_address(1 << 16))
+    d, _ = _desc(src0=_address(0), **ptr)
+    for out in (0, 16, 112, -112):
+        assert lib.ivid_gn_act_forward(ctypes.byref(d), _address(out), _address(1 << 17), None, 0, None) != 0
+        assert "overlaps" in msg(), out
+    for dx in (0, 4096, 4096 + 112):      # x, dy, the end of dy
+        assert lib.ivid_gn_act_backward(ctypes.byref(d), _address(1 << 17), _address(4096), _address(dx), None, _address(1 << 18),
+                                        _address(1 << 18), None, _address(1 << 19), 1 << 16, None) != 0
+        assert "overlaps" in msg(), dx
+    d, _ = _desc(src0=_address(0), C1=8, src1=_address(1024), ld1=16, sn1=64, **ptr)
+    for out in (1024 + 3 * 64 + 16, 1024 - 240):       # the last pixel of the second source, its first from below
+        assert lib.ivid_gn_act_forward(ctypes.byref(d), _address(out), _address(1 << 17), None, 0, None) != 0
+        assert "overlaps" in msg(), out
+    for d0, d1 in ((8192, 8192 + 112), (8192, 1024), (1024 + 16, 8192), (8192, 4096 + 240)):
+        assert lib.ivid_gn_act_backward(ctypes.byref(d), _address(1 << 17), _address(4096), _address(d0), _address(d1), _address(1 << 18),
+                                        _address(1 << 18), None, _address(1 << 19), 1 << 16, None) != 0
+        assert "overlaps" in msg(), (d0, d1)
+    for x, out in ((0, 16), (16, 0), (0, 28), (28, 0)):
+        assert lib.ivid_dropout(0, _address(x), _address(out), 8, 0.5, 1, 2, None, None) != 0
+        assert "overlap" in msg()
+
+
 def test_reference_gradients_are_autograds():
     """The closed-form gradients of functional_ref against automatic differentiation in 64 bits."""
     g = torch.Generator().manual_seed(0)

@@ -402,6 +402,26 @@ def test_autograd_through_leaves_is_refused_under_capture():
     assert F().group_norm_act(x, 8, w, b).requires_grad
 
 
+def test_autograd_behind_a_leaf_is_refused_under_capture():
+    from ivid_amd._lib import IvidHipError
+    leaf = randn(1, 2, 4, 4, 32).requires_grad_()
+    x = leaf * 2
+    w, b = torch.ones(32, device="cuda"), torch.zeros(32, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    refused = 0
+    with torch.cuda.graph(g):
+        for fn in (lambda: F().group_norm_act(x, 8, w, b), lambda: F().dropout(x, 0.5, RNG)):
+            try:
+                fn()
+            except IvidHipError:
+                refused += 1
+        with torch.no_grad():
+            y = F().dropout(F().group_norm_act(x, 8, w, b), 0.5, RNG)
+    assert refused == 2
+    g.replay()
+    assert torch.equal(y, F().dropout(F().group_norm_act(x, 8, w, b), 0.5, RNG))
+
+
 def test_a_rewritten_rng_tensor_is_noticed():
     x = randn(1, 100).requires_grad_()
     rng = torch.tensor([1, 2], device="cuda")
@@ -518,6 +538,24 @@ def test_saved_tensors_may_be_moved_or_recomputed():
         assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("layout", ["offset", "pixel stride", "both strides"])
+def test_saved_tensors_may_come_back_with_other_strides_and_alignment(layout):
+    """The backward pass is cut by the strides and the alignment of the tensors that it gets, not by those of the forward call."""
+    n, hw, c = 2, 1300, 64
+    if layout == "offset":
+        x = randn(3, n * hw * c + 1, dtype=torch.bfloat16)[1:].view(n, hw, c)
+    elif layout == "pixel stride":
+        x = randn(3, n, hw, c + 1, dtype=torch.bfloat16)[..., :c]
+    else:
+        x = randn(3, n, hw + 1, c + 3, dtype=torch.bfloat16)[:, 1:, 3:]
+    x, w, b, dy = x.detach().requires_grad_(), randn(4, c).requires_grad_(), randn(5, c).requires_grad_(), randn(6, n, hw, c, dtype=torch.bfloat16)
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: s, lambda s: s.clone(memory_format=torch.contiguous_format)):
+        y = F().group_norm_act(x, 8, w, b, p=0.1, rng=RNG)
+    want, bound = R.gn_act(x.detach(), 8, w.detach(), b.detach(), p=0.1, rng=RNG, dy=dy)
+    got = dict(zip(("dx", "dweight", "dbias"), torch.autograd.grad(y, [x, w, b], dy)))
+    R.check(got, {k: want[k] for k in got}, bound)
+
+
 def test_a_constant_sample():
     """No variance: xhat is 0 to the rounding of the mean, rstd 1 / sqrt(eps) -- 10^4 with eps = 10^-8 --, and nothing is NaN."""
     x = torch.full((2, 17, 64), 3.0, device="cuda")
@@ -546,6 +584,10 @@ def test_python_entry_points_refuse_what_does_not_fit():
         args = dict(dict(x=x, groups=8, weight=w, bias=b), **kw)
         with pytest.raises(err):
             f.group_norm_act(**args)
+    one = torch.ones(1, device="cuda")
+    for huge in (one.expand(1, (1 << 32) + 4, 1), one.expand((1 << 32) + 4, 1, 1)):      # sizes that would wrap to 4
+        with pytest.raises(ValueError):
+            f.group_norm_act(huge, 1, one, one)
     y, stats = f.group_norm_act_forward(x, 8, w, b)
     for dy, st in ((y[:1], stats), (y.half(), stats), (y, stats[:1]), (y, stats.double()), (y.cpu(), stats)):
         with pytest.raises(ValueError):
