@@ -30,8 +30,9 @@
 //     other while the sums run, with lighter joins: forward 317 -> 255, backward 570 -> 433;
 //   * the group sums published in front of the channel sums: backward 425 -> 374;
 //   * slabs of 64 bytes 255 / 488 where 128 ran 238 / 426; of 256 bytes 302 / 528 where 128 ran 309 / 506 (forward / backward);
-//   * what is left: the vector units are busy 64 % (forward) and 59 % (backward) of the time by the counters, and a workgroup reads, sums,
-//     waits and writes in turn, so that these overlap with memory between workgroups only.
+//   * what is left: the vector units are busy 64 % of the forward's and 68 % of the backward's time by the counters (78 and 72 % with
+//     dropout: 9 more instructions an element, of 20 and 28), and a workgroup reads, sums, waits and writes in turn, so that these
+//     overlap with memory between workgroups only.
 #include <math.h>
 #include <utility>
 #include "common.h"
