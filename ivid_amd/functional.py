@@ -16,6 +16,9 @@ Capturing a training step into a graph: use the `*_forward` / `*_backward` pairs
 capture the operators refuse tensors that require gradients, leaves or not, because accumulating into a leaf whose earlier eager
 graph still lives would make the capturing stream wait for that graph's stream, which ends the process.  For the same reason do
 not capture the backward pass of a graph that was built in eager code.
+
+Small training calls are bound by the host, and half of that is torch's change to its own thread for the backward pass: forward and
+gradients of a 7 x 37 x 23 x 100 tensor take 130 us, 67 under torch.autograd.set_multithreading_enabled(False).
 """
 import ctypes as C
 import math
