@@ -104,7 +104,7 @@ def _dropout(x, p, rng):
 # The backward passes run in autograd's own thread, where Python is several times slower than in the caller's: what can be prepared in
 # the forward call is, and the wrapper that makes them differentiable once is only entered under create_graph.
 def _dropout_grads(ctx, dy):
-    return _dropout(dy, ctx.p, ctx.saved_tensors[0] if ctx.rng is None else ctx.rng), None, None
+    return _dropout(dy, ctx.p, ctx.saved_tensors[0] if ctx.device_rng else ctx.rng), None, None
 
 
 _dropout_grads_once = once_differentiable(_dropout_grads)
@@ -113,10 +113,11 @@ _dropout_grads_once = once_differentiable(_dropout_grads)
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, rng):
-        ctx.p, ctx.rng = p, rng
-        if isinstance(rng, torch.Tensor):
+        ctx.p, ctx.device_rng = p, isinstance(rng, torch.Tensor)      # (rng may be None: p = 0 or an empty x)
+        if ctx.device_rng:
             ctx.save_for_backward(rng)
-            ctx.rng = None
+        else:
+            ctx.rng = rng
         return _dropout(x, p, rng)
 
     @staticmethod

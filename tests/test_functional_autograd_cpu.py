@@ -1,0 +1,47 @@
+"""CPU: what the autograd functions of ivid_amd.functional hand to the library, with the launch itself replaced.  The library's host
+code (scratch sizes, refusals) is the real one; tensors live on the CPU and only the stand-in below touches them."""
+import ctypes
+
+import pytest
+import torch
+
+SIZES = {0: 4, 1: 2, 2: 2}      # bytes of an element by the library's dtype code
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """ivid_amd.functional over CPU tensors.  `launches` collects (name, arguments); a dropout with p = 0 copies, another zeroes."""
+    from ivid_amd import functional as F
+
+    def launch(name, device, *args):
+        F.launches.append((name, args))
+        if name == "ivid_dropout":
+            dtype, src, dst, n, p = args[:5]
+            if p == 0:
+                ctypes.memmove(dst, src, n * SIZES[dtype])
+            else:
+                ctypes.memset(dst, 0, n * SIZES[dtype])
+    monkeypatch.setattr(F, "launches", [], raising=False)
+    monkeypatch.setattr(F, "_check_x", lambda x, name: None)
+    monkeypatch.setattr(F, "_launch", launch)
+    monkeypatch.setattr(F, "_refuse_capture", lambda: None)
+    return F
+
+
+@pytest.mark.parametrize("rng", [None, (1, 2), "tensor"])
+@pytest.mark.parametrize("shape", [(7, 3), (0, 3)], ids=["full", "empty"])
+@pytest.mark.parametrize("p", [0.0, 0.25])
+def test_dropout_has_a_gradient_with_every_form_of_rng(host, p, shape, rng):
+    """p = 0 draws nothing and needs no rng, in the backward pass either; nor has an empty tensor anything to draw."""
+    if rng is None and p > 0 and shape[0]:
+        pytest.skip("p > 0 needs rng")
+    if rng == "tensor":
+        rng = torch.tensor([1, 2])
+    x = torch.randn(shape).requires_grad_()
+    dy = torch.randn(shape)
+    for create_graph in (False, True):
+        y = host.dropout(x, p, rng) if rng is not None else host.dropout(x, p)
+        (dx,) = torch.autograd.grad(y, x, dy, create_graph=create_graph)
+        assert torch.equal(dx, dy if p == 0 else torch.zeros_like(dy))
+    for name, args in host.launches:
+        assert args[4] == p and args[5:] == ((1, 2, None) if isinstance(rng, tuple) and p else (0, 0, rng.data_ptr() if p else None))

@@ -595,3 +595,13 @@ def test_python_entry_points_refuse_what_does_not_fit():
     dy = torch.empty(2 * 4 * 32 + 1, device="cuda")[1:].view(2, 4, 32).copy_(y)      # a gradient that is not on 16 bytes
     for p, q in zip(f.group_norm_act_backward(dy, stats, x, 8, w, b), f.group_norm_act_backward(y, stats, x, 8, w, b)):
         assert (p is None and q is None) or torch.equal(p, q)
+
+
+def test_dropout_without_draws_has_a_gradient():
+    """p = 0 needs no rng, in the backward pass either; an empty tensor has nothing to draw."""
+    for shape, p in (((40, 30), 0.0), ((0, 5), 0.0), ((0, 5), 0.5)):
+        x = torch.empty(shape, device="cuda").normal_().requires_grad_()
+        dy = torch.empty(shape, device="cuda").normal_()
+        y = F().dropout(x, p)
+        (dx,) = torch.autograd.grad(y, x, dy)
+        assert torch.equal(y, x) and torch.equal(dx, dy)
