@@ -113,12 +113,13 @@ _dropout_grads_once = once_differentiable(_dropout_grads)
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, rng):
-        ctx.p, ctx.device_rng = p, isinstance(rng, torch.Tensor)      # (rng may be None: p = 0 or an empty x)
+        y = _dropout(x, p, rng)
+        ctx.p, ctx.device_rng = p, isinstance(rng, torch.Tensor)
         if ctx.device_rng:
             ctx.save_for_backward(rng)
-        else:
-            ctx.rng = rng
-        return _dropout(x, p, rng)
+        else:      # (the caller may rewrite a list; without draws rng may be anything)
+            ctx.rng = tuple(rng) if p and y.numel() else None
+        return y
 
     @staticmethod
     def backward(ctx, dy):
@@ -337,7 +338,7 @@ class _GroupNormAct(torch.autograd.Function):
         call.keep = None        # what saves, offloads or recomputes saved tensors decides over their lives
         if not call.empty:
             call.backward_bytes = call.scratch_bytes(1)
-        ctx.call, ctx.rng = call, None if device_rng else rng
+        ctx.call, ctx.rng = call, tuple(rng) if p and not device_rng else None      # (the caller may rewrite a list)
         return y
 
     @staticmethod

@@ -10,10 +10,13 @@ SIZES = {0: 4, 1: 2, 2: 2}      # bytes of an element by the library's dtype cod
 
 @pytest.fixture
 def host(monkeypatch):
-    """ivid_amd.functional over CPU tensors.  `launches` collects (name, arguments); a dropout with p = 0 copies, another zeroes."""
-    from ivid_amd import functional as F
+    """ivid_amd.functional over CPU tensors.  `launches` collects (name, arguments), a descriptor
+    as it was then; a dropout with p = 0 copies, another zeroes."""
+    from ivid_amd import _lib, functional as F
 
     def launch(name, device, *args):
+        if name.startswith("ivid_gn_act"):
+            args = (_lib.GnActDesc.from_buffer_copy(args[0]._obj),) + args[1:]
         F.launches.append((name, args))
         if name == "ivid_dropout":
             dtype, src, dst, n, p = args[:5]
@@ -45,3 +48,24 @@ def test_dropout_has_a_gradient_with_every_form_of_rng(host, p, shape, rng):
         assert torch.equal(dx, dy if p == 0 else torch.zeros_like(dy))
     for name, args in host.launches:
         assert args[4] == p and args[5:] == ((1, 2, None) if isinstance(rng, tuple) and p else (0, 0, rng.data_ptr() if p else None))
+
+
+def _norm_inputs(n=2, hw=6, c=8, spread=1):
+    """x (strided with spread > 1, so that the backward pass describes it anew), weight, bias; all leaves"""
+    x = torch.randn(n, hw, c * spread)[..., :c].detach().requires_grad_()
+    return x, torch.ones(c).requires_grad_(), torch.zeros(c).requires_grad_()
+
+
+@pytest.mark.parametrize("spread", [1, 2], ids=["in place", "strided"])
+def test_a_rewritten_list_of_seed_and_stream_does_not_reach_the_backward_pass(host, spread):
+    """rng may be any pair of integers; what the forward pass drew with is what the gradient is drawn with."""
+    rng = [5, 6]
+    x, w, b = _norm_inputs(spread=spread)
+    a, y = host.dropout(x, 0.25, rng), host.group_norm_act(x, 2, w, b, p=0.25, rng=rng)
+    rng[0] = 7
+    torch.autograd.grad([a, y], [x, w, b], [torch.ones_like(a), torch.ones_like(y)])
+    drawn = {}
+    for name, args in host.launches:
+        seed = args[5:7] if name == "ivid_dropout" else (args[0].seed, args[0].stream_id)
+        drawn.setdefault(name, []).append(seed)
+    assert drawn == {"ivid_dropout": [(5, 6)] * 2, "ivid_gn_act_forward": [(5, 6)], "ivid_gn_act_backward": [(5, 6)]}
