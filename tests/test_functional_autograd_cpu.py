@@ -69,3 +69,38 @@ def test_a_rewritten_list_of_seed_and_stream_does_not_reach_the_backward_pass(ho
         seed = args[5:7] if name == "ivid_dropout" else (args[0].seed, args[0].stream_id)
         drawn.setdefault(name, []).append(seed)
     assert drawn == {"ivid_dropout": [(5, 6)] * 2, "ivid_gn_act_forward": [(5, 6)], "ivid_gn_act_backward": [(5, 6)]}
+
+
+def test_forward_mode_tangents_are_refused(host):
+    """The kernels propagate no tangent: an output without one would read as a zero derivative."""
+    import torch.autograd.forward_ad as fwd
+    from ivid_amd._lib import IvidHipError
+    F = host
+    n, hw, c = 2, 6, 8
+    t = dict(x=torch.randn(n, hw, c), weight=torch.ones(c), bias=torch.zeros(c), film=torch.zeros(n, 4 * c), skip=torch.randn(n, hw, c))
+    t["weight"], t["bias"] = torch.ones(2 * c), torch.zeros(2 * c)
+    y, stats = F.group_norm_act_forward(groups=2, **t)
+    count = len(F.launches)
+    with fwd.dual_level():
+        for grad in (True, False):      # with gradients enabled or not, for tensors that ask for none
+            with torch.set_grad_enabled(grad):
+                with pytest.raises(IvidHipError, match="tangent"):
+                    F.dropout(fwd.make_dual(t["x"], torch.ones_like(t["x"])), 0.0)
+                for k in t:
+                    dual = dict(t, **{k: fwd.make_dual(t[k], torch.ones_like(t[k]))})
+                    for fn in (F.group_norm_act, F.group_norm_act_forward, lambda **kw: F.group_norm_act_backward(y, stats, **kw)):
+                        with pytest.raises(IvidHipError, match="tangent"):
+                            fn(groups=2, **dual)
+                for k, v in (("dy", y), ("stats", stats)):
+                    args = dict(dict(dy=y, stats=stats), **{k: fwd.make_dual(v, torch.ones_like(v))})
+                    with pytest.raises(IvidHipError, match="tangent"):
+                        F.group_norm_act_backward(groups=2, **args, **t)
+        # a gradient with a tangent, forward over reverse
+        x = t["x"].clone().requires_grad_()
+        for out in (F.dropout(x, 0.0), F.group_norm_act(x, 2, torch.ones(c), torch.zeros(c))):
+            count += 1
+            with pytest.raises(IvidHipError, match="tangent"):
+                torch.autograd.grad(out, x, fwd.make_dual(torch.ones_like(out), torch.ones_like(out)))
+        # tensors without a tangent are as they are elsewhere
+        assert F.group_norm_act(groups=2, **t).shape == y.shape and F.dropout(t["x"], 0.0).shape == t["x"].shape
+    assert len(F.launches) == count + 2
