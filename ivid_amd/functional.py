@@ -243,8 +243,16 @@ class _Call:
         d.seed, d.stream_id, d.rng = _rng_args(rng, self.p, self.device)
         self.keep = (x, skip, weight, bias, film, rng)
 
+    def on(self, x, weight, bias, film, skip, rng):
+        """This call on the tensors that autograd saved, as an object of its own: threads may walk one retained graph at once."""
+        call = object.__new__(_Call)
+        call.__dict__.update(self.__dict__)
+        call.desc = _lib.GnActDesc.from_buffer_copy(self.desc)
+        call.rebind(x, weight, bias, film, skip, rng)
+        return call
+
     def rebind(self, x, weight, bias, film, skip, rng):
-        """bind() for the tensors that autograd saved, which are mostly where they were."""
+        """bind() for tensors that are mostly where they were."""
         if self.in_place and self.strides == (x.stride(), weight.stride(), bias.stride(), None if film is None else film.stride(),
                                               None if skip is None else skip.stride()):
             d = self.desc
@@ -329,10 +337,8 @@ class _Call:
 def _gn_grads(ctx, dy):
     _refuse_tangents(dy)
     x, weight, bias, film, skip, stats, rng = ctx.saved_tensors
-    call = ctx.call
-    call.rebind(x, weight, bias, film, skip, ctx.rng if rng is None else rng)
+    call = ctx.call.on(x, weight, bias, film, skip, ctx.rng if rng is None else rng)
     dx, dskip, dw, db, dfilm = call.gradients(dy, stats, x, weight, bias, film, skip)
-    call.keep = None
     need = ctx.needs_input_grad
     return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None, dfilm if need[3] else None,
             dskip if need[4] else None, None, None, None, None, None)

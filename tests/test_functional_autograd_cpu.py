@@ -1,6 +1,7 @@
 """CPU: what the autograd functions of ivid_amd.functional hand to the library, with the launch itself replaced.  The library's host
 code (scratch sizes, refusals) is the real one; tensors live on the CPU and only the stand-in below touches them."""
 import ctypes
+import threading
 
 import pytest
 import torch
@@ -104,3 +105,41 @@ def test_forward_mode_tangents_are_refused(host):
         # tensors without a tangent are as they are elsewhere
         assert F.group_norm_act(groups=2, **t).shape == y.shape and F.dropout(t["x"], 0.0).shape == t["x"].shape
     assert len(F.launches) == count + 2
+
+
+@pytest.mark.parametrize("spread", [1, 2], ids=["in place", "strided"])
+def test_two_threads_walk_one_retained_graph(host, monkeypatch, spread):
+    """Each backward pass launches on the tensors that it unpacked itself (here filled with the thread's number), or on its own
+    copies of them, and they live until the launch has returned."""
+    x, w, b = _norm_inputs(spread=spread)
+    me = threading.local()
+
+    def unpack(t):
+        return t.clone().fill_(me.number) if spread == 1 else torch.full(t.shape + (2,), float(me.number))[..., 0]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y = host.group_norm_act(x, 2, w, b)
+    both = threading.Barrier(2, timeout=60)
+    seen, failed = {}, []
+
+    def launch(name, device, desc, *args):
+        both.wait()      # both have described their call
+        d = desc._obj
+        seen[me.number] = [ctypes.c_float.from_address(q).value for q in (d.src0, d.gamma, d.beta)]
+        both.wait()
+    monkeypatch.setattr(host, "_launch", launch)
+
+    def walk(number):
+        me.number = number
+        try:
+            with torch.autograd.set_multithreading_enabled(False):
+                torch.autograd.grad(y, [x, w, b], torch.ones_like(y), retain_graph=True)
+        except Exception as e:      # noqa: BLE001
+            failed.append(e)
+            both.abort()
+    threads = [threading.Thread(target=walk, args=(i,)) for i in (1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not failed
+    assert seen == {i: [float(i)] * 3 for i in (1, 2)}
