@@ -213,7 +213,7 @@ class _Call:
         hw = numel // (n * c0) if numel else 0
         if max(n, hw, c) > _INT_MAX:      # the descriptor's ints would wrap without a word
             raise ValueError(f"[{n}, {hw}, {c}] is too large: every size must be below 2^31")
-        self.device, self.dtype = dev, dtype
+        self.device, self.index, self.dtype = dev, x.get_device(), dtype
         self.film_dtype = film.dtype if film is not None else None
         self.shape = shape if c1 == 0 else shape[:-1] + (c,)
         self.n, self.c0, self.c1, self.c, self.groups, self.p = n, c0, c1, c, groups, p
@@ -245,6 +245,17 @@ class _Call:
 
     def on(self, x, weight, bias, film, skip, rng):
         """This call on the tensors that autograd saved, as an object of its own: threads may walk one retained graph at once."""
+        c, index, dtype, shape = self.c, self.index, self.dtype, self.shape
+        if skip is not None:
+            shape = shape[:-1] + (self.c0,)
+        ok = (x.shape == shape and weight.shape == bias.shape == (c,) and x.dtype is dtype and weight.dtype is bias.dtype is torch.float32
+              and x.get_device() == weight.get_device() == bias.get_device() == index)
+        if film is not None:
+            ok = ok and film.shape == (self.n, 2 * c) and film.dtype is self.film_dtype and film.get_device() == index
+        if skip is not None:
+            ok = ok and skip.shape == shape[:-1] + (self.c1,) and skip.dtype is dtype and skip.get_device() == index
+        if not ok:      # the launch would read past its end
+            raise ValueError("a saved tensor came back with another type, shape or device")
         call = object.__new__(_Call)
         call.__dict__.update(self.__dict__)
         call.desc = _lib.GnActDesc.from_buffer_copy(self.desc)
@@ -265,7 +276,7 @@ class _Call:
             if before != (d.src0, d.src1):
                 self.backward_bytes = None
             if d.rng:
-                d.rng = rng.data_ptr()
+                d.rng = _rng_args(rng, self.p, self.device)[2]
         else:
             self.bind(x, weight, bias, film, skip, rng)
 
@@ -297,12 +308,12 @@ class _Call:
     def backward(self, dy, stats):
         if dy.shape != self.shape or dy.dtype != self.dtype or dy.device != self.device:
             raise ValueError(f"dy must be {tuple(self.shape)} {self.dtype} on {self.device}")
-        if stats.shape != (self.n, self.groups, 2) or stats.dtype != torch.float32 or stats.device != self.device:
-            raise ValueError("stats must be what the forward call returned")
         x, skip, weight, bias, film, _ = self.keep
         return self.gradients(dy, stats.contiguous(), x, weight, bias, film, skip)
 
     def gradients(self, dy, stats, x, weight, bias, film, skip):
+        if stats.shape != (self.n, self.groups, 2) or stats.dtype != torch.float32 or stats.device != self.device:
+            raise ValueError("stats must be what the forward call returned")
         if not dy.is_contiguous():
             dy = dy.contiguous()
         if dy.data_ptr() % 16:

@@ -143,3 +143,33 @@ def test_two_threads_walk_one_retained_graph(host, monkeypatch, spread):
         t.join(120)
     assert not failed
     assert seen == {i: [float(i)] * 3 for i in (1, 2)}
+
+
+@pytest.mark.parametrize("spread", [1, 2], ids=["in place", "strided"])
+@pytest.mark.parametrize("which", ["x", "skip", "weight", "bias", "film", "stats"])
+def test_saved_tensors_that_come_back_as_others_are_refused(host, which, spread):
+    """A hook that unpacks another type or shape than it was given: the launch would read past their ends."""
+    n, hw, c = 2, 6, 8
+    x, _, _ = _norm_inputs(n, hw, c, spread)
+    t = dict(x=x, skip=torch.randn(n, hw, c), weight=torch.ones(2 * c), bias=torch.zeros(2 * c), film=torch.zeros(n, 4 * c))
+    for bad in (lambda s: s.half(), lambda s: s[:1], lambda s: s.unsqueeze(0)):
+        order = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda s: (len(order), order.append(1), s)[::2],
+                                                      lambda k: bad(k[1]) if k[0] == ["x", "weight", "bias", "film", "skip", "stats"].index(which) else k[1]):
+            y = host.group_norm_act(groups=2, **t)
+        host.launches.clear()
+        with pytest.raises((ValueError, RuntimeError), match="saved|stats"):
+            torch.autograd.grad(y, x, torch.ones_like(y))
+        assert not host.launches
+
+
+def test_a_saved_rng_that_comes_back_as_another_is_refused(host):
+    x, w, b = _norm_inputs()
+    for bad in (lambda s: s.int(), lambda s: s[:1], lambda s: s.to("meta")):
+        with torch.autograd.graph.saved_tensors_hooks(lambda s: s, lambda s: bad(s) if s.dtype == torch.int64 else s):
+            ys = [host.group_norm_act(x, 2, w, b, p=0.5, rng=torch.tensor([1, 2])), host.dropout(x, 0.5, torch.tensor([1, 2]))]
+        host.launches.clear()
+        for y in ys:
+            with pytest.raises(ValueError, match="rng"):
+                torch.autograd.grad(y, x, torch.ones_like(y))
+        assert not host.launches

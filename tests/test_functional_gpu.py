@@ -605,3 +605,21 @@ def test_dropout_without_draws_has_a_gradient():
         y = F().dropout(x, p)
         (dx,) = torch.autograd.grad(y, x, dy)
         assert torch.equal(y, x) and torch.equal(dx, dy)
+
+
+def test_saved_tensors_that_come_back_elsewhere_are_refused():
+    t = gn_inputs(141, (2, 6, 6), 32, 32, torch.bfloat16, "f32")
+    x = t["x"].requires_grad_()
+    for name in ("x", "skip", "weight", "bias", "film", "stats"):
+        shape = t[name].shape if name in t else (2, 8, 2)
+        seen = []
+
+        def unpack(s, shape=shape, name=name, seen=seen):
+            if s.shape == shape and (name != "bias" or seen):      # (weight and bias have one shape; the weight comes first)
+                return s.cpu()
+            seen.extend([1] * (s.dim() == 1))
+            return s
+        with torch.autograd.graph.saved_tensors_hooks(lambda s: s, unpack):
+            y = F().group_norm_act(x, 8, t["weight"], t["bias"], film=t["film"], skip=t["skip"])
+        with pytest.raises(ValueError):
+            torch.autograd.grad(y, x, torch.ones_like(y))
