@@ -309,11 +309,12 @@ class _Call:
         if dy.shape != self.shape or dy.dtype != self.dtype or dy.device != self.device:
             raise ValueError(f"dy must be {tuple(self.shape)} {self.dtype} on {self.device}")
         x, skip, weight, bias, film, _ = self.keep
-        return self.gradients(dy, stats.contiguous(), x, weight, bias, film, skip)
+        return self.gradients(dy, stats, x, weight, bias, film, skip)
 
     def gradients(self, dy, stats, x, weight, bias, film, skip):
         if stats.shape != (self.n, self.groups, 2) or stats.dtype != torch.float32 or stats.device != self.device:
             raise ValueError("stats must be what the forward call returned")
+        stats = stats.contiguous()
         if not dy.is_contiguous():
             dy = dy.contiguous()
         if dy.data_ptr() % 16:

@@ -173,3 +173,18 @@ def test_a_saved_rng_that_comes_back_as_another_is_refused(host):
             with pytest.raises(ValueError, match="rng"):
                 torch.autograd.grad(y, x, torch.ones_like(y))
         assert not host.launches
+
+
+def test_statistics_that_come_back_with_other_strides(host, monkeypatch):
+    x, w, b = _norm_inputs(n=3)
+    values = torch.arange(12.0).reshape(3, 2, 2)
+
+    def unpack(t):      # the statistics have a shape of their own
+        return values.clone().transpose(0, 2).contiguous().transpose(0, 2) if t.shape == values.shape else t
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y = host.group_norm_act(x, 2, w, b)
+    seen = []
+    monkeypatch.setattr(host, "_launch", lambda name, device, desc, stats, *args: seen.append(
+        [ctypes.c_float.from_address(stats + 4 * i).value for i in range(12)]))
+    torch.autograd.grad(y, x, torch.ones_like(y))
+    assert seen == [values.reshape(-1).tolist()]

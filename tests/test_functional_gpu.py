@@ -623,3 +623,19 @@ def test_saved_tensors_that_come_back_elsewhere_are_refused():
             y = F().group_norm_act(x, 8, t["weight"], t["bias"], film=t["film"], skip=t["skip"])
         with pytest.raises(ValueError):
             torch.autograd.grad(y, x, torch.ones_like(y))
+
+
+@pytest.mark.parametrize("dtype", DTS, ids=["f32", "bf16", "f16"])
+def test_saved_tensors_may_come_back_transposed_in_memory(dtype):
+    """Every saved tensor, the statistics among them, with its first and last dimension swapped in memory."""
+    t = gn_inputs(151, (3, 9, 7), 24, 16, dtype, "f32")
+    dy = randn(152, 3, 9, 7, 40, dtype=dtype)
+    names = ("x", "skip", "weight", "bias", "film")
+    leaves = {k: t[k].requires_grad_() for k in names}
+    kw = dict(p=0.2, rng=RNG)
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: s, lambda s: s.transpose(0, -1).contiguous().transpose(0, -1)):
+        y = F().group_norm_act(x=leaves["x"], groups=8, weight=leaves["weight"], bias=leaves["bias"], film=leaves["film"],
+                               skip=leaves["skip"], **kw)
+    got = dict(zip(["d" + k for k in names], torch.autograd.grad(y, list(leaves.values()), dy)), y=y)
+    want, bound = R.gn_act(t["x"], 8, t["weight"], t["bias"], film=t["film"], skip=t["skip"], dy=dy, **kw)
+    R.check(got, {k: want[k] for k in got}, bound)
