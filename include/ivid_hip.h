@@ -285,8 +285,9 @@ int ivid_gn_apply_p(int dtype, const void* src0, const void* src0_lo, int C0, co
  *   y = drop(act(u * (1 + scale) + shift)),  u = xhat * gamma + beta,  xhat = (x - mean) * rstd
  * x = cat[src0, src1] over channels, N samples of HW pixels; mean and biased variance per (sample, group) in fp32 or wider;
  * act 0 none, 1 SiLU; drop as in ivid_dropout, element index = row-major index in the [N,HW,C0+C1] output.
- * Any N, HW >= 1, any C0 + C1 divisible by groups; src0, src1, gamma, beta and film may be aligned to an element only, every other
- * pointer of a tensor to 16 bytes.  Outputs and scratch overlap neither the inputs nor each other (not even in place). */
+ * N, HW >= 1, any C0 + C1 <= 2^24 divisible by groups.  Refused: calls that are cut into 2^24 tiles or more (a sample takes one at
+ * least) and calls with N * ceil((C0 + C1) / 64) >= 2^24.  src0, src1, gamma, beta and film may be aligned to an element only, every
+ * other pointer of a tensor to 16 bytes.  Outputs and scratch overlap neither the inputs nor each other (not even in place). */
 typedef struct {
   int dtype;                              /* IVID_F32, IVID_BF16 or IVID_F16: src, out, dy, dsrc */
   int N, HW, C0, C1, groups, act;         /* C1 = 0 and src1 = NULL: one source */

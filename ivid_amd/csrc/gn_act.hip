@@ -122,6 +122,7 @@ struct Cut {
   int K, GS, logW;          // tiles of a cluster, groups of a slab, log2 of the lanes per group (a team) in the reductions
   int seg, logseg;          // channels of a run: the largest power of two that divides the group and the piece
   int polls, phase;
+  int block0;               // first workgroup of this launch (forward)
   Div by_nslab, by_K, by_PP, by_Cg, by_runs;
 };
 
@@ -448,7 +449,8 @@ __global__ __launch_bounds__(NT, 4) void gn_act_fwd_kernel(GnArgs a, char* __res
   __shared__ double2 tot[MAX_GS];
   __shared__ int missing;
   const Cut& q = a.cut;
-  const int rest = q.by_K.of(blockIdx.x), me = blockIdx.x - rest * q.K;      // a cluster's tiles start together
+  const int block = q.block0 + blockIdx.x;
+  const int rest = q.by_K.of(block), me = block - rest * q.K;      // a cluster's tiles start together
   const int n = q.by_nslab.of(rest), slab = rest - n * q.nslab;
   const Tile t = tile_of<VE>(a, slab, me, threadIdx.x);
 
@@ -1012,7 +1014,7 @@ int cut_up(const ivid_gn_act_desc* d, bool backward, GnArgs* a, int* ve_out) {
   }
   q.polls = d->max_polls > 0 ? d->max_polls : MAX_POLLS;
   *ve_out = ve;
-  const double tiles = (double)d->N * q.nslab * q.krows * q.kcols;
+  const double tiles = (double)d->N * q.nslab * q.krows * q.kcols;      // 2^24 - 1 are what Div takes, and 2^32 threads of a backward pass
   q.K = tiles < (1 << 24) ? q.krows * q.kcols : 0;
   if (!q.K || (long long)d->N * ((C + 63) / 64) >= (1 << 24))
     return ivid_set_error("gn_act: too many tiles for one launch", hipSuccess);
@@ -1127,7 +1129,11 @@ extern "C" int ivid_gn_act_forward(const ivid_gn_act_desc* d, void* out, float* 
   if (scratch_bytes < s.total || (s.total && (!scratch || ((uintptr_t)scratch & 15)))) return ivid_set_error("gn_act: scratch too small or misaligned", hipSuccess);
   hipStream_t st = (hipStream_t)stream;
   if (int e = clear_words(s, scratch, st)) return e;
-  const dim3 grid((unsigned)((long long)d->N * a.cut.nslab * a.cut.K));
+  // A grid of 2^32 threads is dropped without an error: several launches, and no cluster that waits is cut in two.
+  const int tiles = d->N * a.cut.nslab * a.cut.K;
+  int most = (int)(0xFFFFFFFFu / NT_FWD);
+  if (a.cut.K <= MAX_K) most -= most % a.cut.K;
+  dim3 grid;
 #define LAUNCH(T, VE, NV) \
   hipLaunchKernelGGL((gn_act_fwd_kernel<NT_FWD, T, VE, NV>), grid, dim3(NT_FWD), 0, st, a, (char*)out, stats, (unsigned long long*)scratch, \
                      (const double2*)((char*)scratch + s.words))
@@ -1151,14 +1157,17 @@ extern "C" int ivid_gn_act_forward(const ivid_gn_act_desc* d, void* out, float* 
     else LAUNCH_NARROW(T, 1);                     \
   } while (0)
   run_phases<NT_FWD, true>(a, d, ve, s, scratch, st, [&] {
-    if (d->dtype == IVID_F32) {
-      if (ve == 4) LAUNCH_NV(float, 4);
-      else if (ve == 2) LAUNCH_NARROW(float, 2);
-      else LAUNCH_NARROW(float, 1);
-    } else if (d->dtype == IVID_BF16) {
-      LAUNCH16(__bf16);
-    } else {
-      LAUNCH16(_Float16);
+    for (a.cut.block0 = 0; a.cut.block0 < tiles; a.cut.block0 += most) {
+      grid = dim3((unsigned)(tiles - a.cut.block0 < most ? tiles - a.cut.block0 : most));
+      if (d->dtype == IVID_F32) {
+        if (ve == 4) LAUNCH_NV(float, 4);
+        else if (ve == 2) LAUNCH_NARROW(float, 2);
+        else LAUNCH_NARROW(float, 1);
+      } else if (d->dtype == IVID_BF16) {
+        LAUNCH16(__bf16);
+      } else {
+        LAUNCH16(_Float16);
+      }
     }
   });
 #undef LAUNCH_NV

@@ -639,3 +639,26 @@ def test_saved_tensors_may_come_back_transposed_in_memory(dtype):
     got = dict(zip(["d" + k for k in names], torch.autograd.grad(y, list(leaves.values()), dy)), y=y)
     want, bound = R.gn_act(t["x"], 8, t["weight"], t["bias"], film=t["film"], skip=t["skip"], dy=dy, **kw)
     R.check(got, {k: want[k] for k in got}, bound)
+
+
+def test_more_samples_than_one_launch_holds():
+    """2^23 + 13 samples of a tile each: the forward pass takes two launches, and every sample is what it is in a call of fewer."""
+    n, c = (1 << 23) + 13, 8
+    x = torch.empty(n, c, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(1))
+    w, b = 1 + 0.2 * randn(2, c), 0.2 * randn(3, c)
+    y, stats = F().group_norm_act_forward(x, 1, w, b, p=0.25, rng=RNG)
+    half = 1 << 22
+    for i in range(0, n, half):
+        y1, stats1 = F().group_norm_act_forward(x[i:i + half], 1, w, b)
+        kept = y[i:i + half] != 0
+        assert torch.equal(stats[i:i + half], stats1)
+        assert abs(kept.float().mean().item() - 0.75) < 0.01
+    for i in (0, half, (1 << 23) - 40, n - 64):
+        want, bound = R.gn_act(x[i:i + 64], 1, w, b)
+        f = torch.from_numpy((R.draws(64 * c, RNG, i * c) >= R.threshold(0.25)) * (4 / 3)).reshape(64, c)
+        bound["y"], want["y"] = bound["y"] * f + 2 * R.U * (want["y"] * f).abs(), want["y"] * f
+        R.check(dict(y=y[i:i + 64], stats=stats[i:i + 64]), want, bound)
+    dy = torch.ones_like(x)
+    dx = F().group_norm_act_backward(dy, stats, x, 1, w, b, p=0.25, rng=RNG)[0]
+    del y, dy
+    assert torch.isfinite(dx[::4099]).all()
