@@ -654,11 +654,44 @@ def test_more_samples_than_one_launch_holds():
         assert torch.equal(stats[i:i + half], stats1)
         assert abs(kept.float().mean().item() - 0.75) < 0.01
     for i in (0, half, (1 << 23) - 40, n - 64):
-        want, bound = R.gn_act(x[i:i + 64], 1, w, b)
-        f = torch.from_numpy((R.draws(64 * c, RNG, i * c) >= R.threshold(0.25)) * (4 / 3)).reshape(64, c)
+        count = min(64, n - i)
+        want, bound = R.gn_act(x[i:i + count], 1, w, b)
+        f = torch.from_numpy((R.draws(count * c, RNG, i * c) >= R.threshold(0.25)) * (4 / 3)).reshape(count, c)
         bound["y"], want["y"] = bound["y"] * f + 2 * R.U * (want["y"] * f).abs(), want["y"] * f
-        R.check(dict(y=y[i:i + 64], stats=stats[i:i + 64]), want, bound)
+        R.check(dict(y=y[i:i + count], stats=stats[i:i + count]), want, bound)
     dy = torch.ones_like(x)
     dx = F().group_norm_act_backward(dy, stats, x, 1, w, b, p=0.25, rng=RNG)[0]
     del y, dy
     assert torch.isfinite(dx[::4099]).all()
+
+
+def test_parameter_gradients_over_many_tiles():
+    """One sample of 2^26 pixels, 16384 tiles that are all alike: their sums are equal terms, whose additions all round the same way.
+    Every sum is 16384 times that over one tile, so is every bound."""
+    tile, count = 4096, 1 << 14
+    x = randn(1, 1, tile, 1, dtype=torch.bfloat16)
+    dy = (1 + 0.5 * x.float() + 0.25 * randn(2, 1, tile, 1)).to(torch.bfloat16)
+    w, b, film = 1 + 0.2 * randn(3, 1), 0.2 * randn(4, 1), 0.3 * randn(5, 1, 2)
+    want, bound = R.gn_act(x, 1, w, b, film=film, dy=dy)
+    whole = lambda t: t.expand(count, tile, 1).reshape(1, count * tile, 1)
+    y, stats = F().group_norm_act_forward(whole(x), 1, w, b, film=film)
+    dx, _, dw, db, dfilm = F().group_norm_act_backward(whole(dy), stats, whole(x), 1, w, b, film=film)
+    for i in (0, tile * 5461, tile * (count - 1)):
+        R.check(dict(y=y[:, i:i + tile], dx=dx[:, i:i + tile], stats=stats), {k: want[k] for k in ("y", "dx", "stats")}, bound)
+    got = dict(dweight=dw, dbias=db, dfilm=dfilm)
+    print("worst ratio", R.check(got, {k: want[k] * count for k in got}, {k: bound[k] * count for k in got}))
+
+
+def test_parameter_gradients_over_many_samples():
+    """2^22 samples that are all alike, one pixel each; the same argument."""
+    n, c = 1 << 22, 8
+    x, dy = randn(1, 1, c), torch.tensor([[1.1, 0.7, 1.9, 0.3, 1.3, 1.23, 0.9, 1.7]], device="cuda")
+    w, b = 1 + 0.2 * randn(3, c), 0.2 * randn(4, c)
+    want, bound = R.gn_act(x, 1, w, b, dy=dy, act="none")
+    y, stats = F().group_norm_act_forward(x.expand(n, c), 1, w, b, act="none")
+    dx, _, dw, db, _ = F().group_norm_act_backward(dy.expand(n, c), stats, x.expand(n, c), 1, w, b, act="none")
+    for t in (y, dx, stats):
+        assert torch.equal(t, t[:1].expand_as(t))
+    R.check(dict(y=y[:1], dx=dx[:1], stats=stats[:1]), {k: want[k] for k in ("y", "dx", "stats")}, bound)
+    got = dict(dweight=dw, dbias=db)
+    print("worst ratio", R.check(got, {k: want[k] * n for k in got}, {k: bound[k] * n for k in got}))
