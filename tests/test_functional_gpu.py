@@ -695,3 +695,59 @@ def test_parameter_gradients_over_many_samples():
     R.check(dict(y=y[:1], dx=dx[:1], stats=stats[:1]), {k: want[k] for k in ("y", "dx", "stats")}, bound)
     got = dict(dweight=dw, dbias=db)
     print("worst ratio", R.check(got, {k: want[k] * n for k in got}, {k: bound[k] * n for k in got}))
+
+
+@pytest.mark.parametrize("dtype", DTS, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape,c0,c1,groups,film,p", [((2, 1100003), 1, 1, 2, "f32", 0.1), ((1, 2200003), 1, 0, 1, None, 0.0)], ids=["skip", "one_channel"])
+def test_more_tiles_than_one_launch_exchanges(shape, c0, c1, groups, film, p, dtype):
+    """A sample of more than 256 tiles takes two launches, sums and results, in both directions."""
+    t = gn_inputs(161, shape, c0, c1, dtype, film, offset=2.0)
+    dy = 0.5 + randn(162, *shape, c0 + c1)
+    dy = dy.to(dtype)
+    kw = dict(act="silu", p=p, rng=RNG if p else None)
+    want, bound = R.gn_act(t["x"], groups, t["weight"], t["bias"], film=t["film"], skip=t["skip"], dy=dy, **kw)
+    got = run_gn(t, groups, dy, **kw)
+    print("worst ratio", R.check(got, want, bound))
+
+
+def test_more_tiles_than_one_launch_exchanges_in_several_slabs():
+    t = gn_inputs(171, (1, 270001), 64, 0, torch.float32, None)
+    dy = 0.5 + randn(172, 1, 270001, 64)
+    want, bound = R.gn_act(t["x"], 32, t["weight"], t["bias"], dy=dy)
+    print("worst ratio", R.check(run_gn(t, 32, dy), want, bound))
+
+
+@pytest.mark.parametrize("dtype", DTS, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape,c0,c1,film", [((40, 200), 5000, 0, "f32"), ((24, 150), 1000, 3096, "same")], ids=["c5000", "skip"])
+def test_a_workgroup_that_stops_waiting_in_a_group_of_several_column_chunks(shape, c0, c1, film, dtype, monkeypatch):
+    """One poll, and more workgroups than the chip holds: a workgroup adds up tiles of other channels than its own and has to come
+    back to its own coefficients."""
+    t = gn_inputs(181, shape, c0, c1, dtype, film)
+    dy = randn(182, *shape, c0 + c1, dtype=dtype)
+    ref = run_gn(t, 1, dy, p=0.1, rng=RNG)
+    monkeypatch.setattr(F(), "_MAX_POLLS", 1)
+    for _ in range(3):
+        got = run_gn(t, 1, dy, p=0.1, rng=RNG)
+        for k in ref:
+            assert torch.equal(ref[k], got[k]), k
+    one = {k: v[:1] if v is not None and k in ("x", "skip", "film") else v for k, v in t.items()}
+    want, bound = R.gn_act(one["x"], 1, t["weight"], t["bias"], film=one["film"], skip=one["skip"], dy=dy[:1], p=0.1, rng=RNG)
+    R.check({k: v[:1] for k, v in ref.items() if k not in ("dweight", "dbias")}, {k: v for k, v in want.items() if k not in ("dweight", "dbias")}, bound)
+
+
+@pytest.mark.parametrize("dtype", DTS, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape,c0,c1,groups", [((9, 37, 23), 100, 0, 20), ((7, 77), 36, 0, 6), ((5, 13, 11), 33, 0, 3), ((5, 40, 41), 18, 30, 6),
+                                                ((3, 90, 91), 64, 0, 32), ((300, 1), 24, 0, 3)])
+def test_independent_of_the_batch_at_odd_sizes(shape, c0, c1, groups, dtype):
+    """A sample alone, as a view of the batch or as a copy, gives the bits that it gives among others."""
+    t = gn_inputs(191, shape, c0, c1, dtype, "f32")
+    dy = randn(192, *shape, c0 + c1, dtype=dtype)
+    whole = run_gn(t, groups, dy)
+    for i in (0, 1, shape[0] - 1):
+        for copy in (False, True):
+            pick = lambda v: v[i:i + 1].clone() if copy else v[i:i + 1]
+            one = {k: pick(v) if v is not None and k in ("x", "skip", "film") else v for k, v in t.items()}
+            got = run_gn(one, groups, pick(dy))
+            for k in whole:
+                if k not in ("dweight", "dbias"):
+                    assert torch.equal(whole[k][i:i + 1], got[k]), (k, i, copy)
