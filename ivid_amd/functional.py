@@ -75,8 +75,8 @@ def _launch(name, device, *args):
     if fn is None:
         fn = _entry[name] = getattr(_lib.load(), name)
     index = device.index
-    # (the raw getter is torch.cuda.current_stream(index).cuda_stream without its 2 us)
-    if index == torch.cuda.current_device():
+    # (the raw getters are torch.cuda.current_device() and torch.cuda.current_stream(index).cuda_stream without their 2 us)
+    if index == torch._C._cuda_getDevice():
         status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
@@ -114,7 +114,8 @@ def _dropout(x, p, rng):
 # The backward passes run in autograd's own thread, where Python is several times slower than in the caller's: what can be prepared in
 # the forward call is, and the wrapper that makes them differentiable once is only entered under create_graph.
 def _dropout_grads(ctx, dy):
-    _refuse_tangents(dy)
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents(dy)
     return _dropout(dy, ctx.p, ctx.saved_tensors[0] if ctx.device_rng else ctx.rng), None, None
 
 
@@ -214,8 +215,12 @@ class _Call:
         if max(n, hw, c) > _INT_MAX:      # the descriptor's ints would wrap without a word
             raise ValueError(f"[{n}, {hw}, {c}] is too large: every size must be below 2^31")
         self.device, self.index, self.dtype = dev, x.get_device(), dtype
-        self.film_dtype = film.dtype if film is not None else None
+        if film is not None:
+            self.film_shape, self.film_dtype = film.shape, film.dtype
+        if c1:
+            self.skip_shape = skip.shape
         self.shape = shape if c1 == 0 else shape[:-1] + (c,)
+        self.x_shape, self.c_shape, self.stats_shape = shape, (c,), (n, groups, 2)
         self.n, self.c0, self.c1, self.c, self.groups, self.p = n, c0, c1, c, groups, p
         self.empty = numel == 0
         d = self.desc = _lib.GnActDesc(_DTYPES[dtype], n, hw, c0, c1, groups, _ACTS[act])
@@ -225,58 +230,47 @@ class _Call:
     def bind(self, x, weight, bias, film, skip, rng):
         """Point the descriptor at these tensors (of the shapes and types checked in front), which the caller keeps alive."""
         d = self.desc
-        self.backward_bytes = None      # depends on strides and alignment
-        self.strides = (x.stride(), weight.stride(), bias.stride(), None if film is None else film.stride(),
-                        None if skip is None else skip.stride())
         self.in_place = (x.is_contiguous() and weight.is_contiguous() and bias.is_contiguous()
                          and (film is None or film.is_contiguous()) and (skip is None or skip.is_contiguous()))
         x, d.ld0, d.sn0 = _pixels(x)
         if skip is not None:
             skip, d.ld1, d.sn1 = _pixels(skip)
-            d.src1 = skip.data_ptr()
         weight, bias = weight.contiguous(), bias.contiguous()
-        d.src0, d.gamma, d.beta = x.data_ptr(), weight.data_ptr(), bias.data_ptr()
         if film is not None:
             if film.stride(1) != 1:
                 film = film.contiguous()
-            d.film, d.film_ld, d.film_dtype = film.data_ptr(), film.stride(0), _DTYPES[film.dtype]
+            d.film_ld, d.film_dtype = film.stride(0), _DTYPES[film.dtype]
+        self.point((x.data_ptr(), None if skip is None else skip.data_ptr(), weight.data_ptr(), bias.data_ptr(),
+                    None if film is None else film.data_ptr()))
         d.seed, d.stream_id, d.rng = _rng_args(rng, self.p, self.device)
+        self.device_rng = d.rng is not None
         self.keep = (x, skip, weight, bias, film, rng)
 
-    def on(self, x, weight, bias, film, skip, rng):
-        """This call on the tensors that autograd saved, as an object of its own: threads may walk one retained graph at once."""
-        c, index, dtype, shape = self.c, self.index, self.dtype, self.shape
-        if skip is not None:
-            shape = shape[:-1] + (self.c0,)
-        ok = (x.shape == shape and weight.shape == bias.shape == (c,) and x.dtype is dtype and weight.dtype is bias.dtype is torch.float32
-              and x.get_device() == weight.get_device() == bias.get_device() == index)
-        if film is not None:
-            ok = ok and film.shape == (self.n, 2 * c) and film.dtype is self.film_dtype and film.get_device() == index
-        if skip is not None:
-            ok = ok and skip.shape == shape[:-1] + (self.c1,) and skip.dtype is dtype and skip.get_device() == index
-        if not ok:      # the launch would read past its end
-            raise ValueError("a saved tensor came back with another type, shape or device")
-        call = object.__new__(_Call)
-        call.__dict__.update(self.__dict__)
-        call.desc = _lib.GnActDesc.from_buffer_copy(self.desc)
-        call.rebind(x, weight, bias, film, skip, rng)
-        return call
+    def point(self, at):
+        d = self.desc
+        self.at = d.src0, d.src1, d.gamma, d.beta, d.film = at
+        self.backward_bytes = None      # depends on strides and alignment
 
     def rebind(self, x, weight, bias, film, skip, rng):
-        """bind() for tensors that are mostly where they were."""
-        if self.in_place and self.strides == (x.stride(), weight.stride(), bias.stride(), None if film is None else film.stride(),
-                                              None if skip is None else skip.stride()):
-            d = self.desc
-            before = d.src0, d.src1
-            d.src0, d.gamma, d.beta = x.data_ptr(), weight.data_ptr(), bias.data_ptr()
-            if film is not None:
-                d.film = film.data_ptr()
-            if skip is not None:
-                d.src1 = skip.data_ptr()
-            if before != (d.src0, d.src1):
-                self.backward_bytes = None
-            if d.rng:
-                d.rng = _rng_args(rng, self.p, self.device)[2]
+        """bind() for the tensors that autograd saved, which are mostly where they were.  A hook may unpack others."""
+        index = self.index
+        same = (x.shape == self.x_shape and x.dtype is self.dtype and x.get_device() == index
+                and weight.shape == bias.shape == self.c_shape and weight.dtype is bias.dtype is torch.float32
+                and weight.get_device() == bias.get_device() == index)
+        if film is not None:
+            same = same and film.shape == self.film_shape and film.dtype is self.film_dtype and film.get_device() == index
+        if skip is not None:
+            same = same and skip.shape == self.skip_shape and skip.dtype is self.dtype and skip.get_device() == index
+        if not same:      # the launch would read past its end
+            raise ValueError("a saved tensor came back with another type, shape or device")
+        if self.in_place and (x.is_contiguous() and weight.is_contiguous() and bias.is_contiguous()
+                              and (film is None or film.is_contiguous()) and (skip is None or skip.is_contiguous())):
+            at = (x.data_ptr(), None if skip is None else skip.data_ptr(), weight.data_ptr(), bias.data_ptr(),
+                  None if film is None else film.data_ptr())
+            if at != self.at:
+                self.point(at)
+            if self.device_rng:
+                self.desc.rng = _rng_args(rng, self.p, self.device)[2]
         else:
             self.bind(x, weight, bias, film, skip, rng)
 
@@ -298,23 +292,27 @@ class _Call:
 
     def forward(self):
         y = torch.empty(self.shape, dtype=self.dtype, device=self.device)
-        stats = torch.empty((self.n, self.groups, 2), dtype=torch.float32, device=self.device)
+        stats = torch.empty(self.stats_shape, dtype=torch.float32, device=self.device)
         if self.empty:
             return y, stats.zero_()
         ptr, nbytes, buf = self.scratch(0)
         _launch("ivid_gn_act_forward", self.device, C.byref(self.desc), y.data_ptr(), stats.data_ptr(), ptr, nbytes)
         return y, stats
 
-    def backward(self, dy, stats):
+    def check_gradient(self, dy):
         if dy.shape != self.shape or dy.dtype != self.dtype or dy.device != self.device:
             raise ValueError(f"dy must be {tuple(self.shape)} {self.dtype} on {self.device}")
+
+    def backward(self, dy, stats):
+        self.check_gradient(dy)
         x, skip, weight, bias, film, _ = self.keep
         return self.gradients(dy, stats, x, weight, bias, film, skip)
 
     def gradients(self, dy, stats, x, weight, bias, film, skip):
-        if stats.shape != (self.n, self.groups, 2) or stats.dtype != torch.float32 or stats.device != self.device:
+        if stats.shape != self.stats_shape or stats.dtype is not torch.float32 or stats.get_device() != self.index:
             raise ValueError("stats must be what the forward call returned")
-        stats = stats.contiguous()
+        if not stats.is_contiguous():
+            stats = stats.contiguous()
         if not dy.is_contiguous():
             dy = dy.contiguous()
         if dy.data_ptr() % 16:
@@ -347,10 +345,22 @@ class _Call:
 
 
 def _gn_grads(ctx, dy):
-    _refuse_tangents(dy)
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents(dy)
     x, weight, bias, film, skip, stats, rng = ctx.saved_tensors
-    call = ctx.call.on(x, weight, bias, film, skip, ctx.rng if rng is None else rng)
+    if rng is None:
+        rng = ctx.rng
+    try:
+        call = ctx.calls.pop()      # (one step under the interpreter's lock: threads may walk one retained graph at once)
+    except IndexError:
+        groups, act, eps, p = ctx.args
+        call = _Call(x, groups, weight, bias, film, skip, act, eps, p, rng)
+        call.check_gradient(dy)
+    else:
+        call.rebind(x, weight, bias, film, skip, rng)
     dx, dskip, dw, db, dfilm = call.gradients(dy, stats, x, weight, bias, film, skip)
+    call.keep = None
+    ctx.calls.append(call)
     need = ctx.needs_input_grad
     return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None, dfilm if need[3] else None,
             dskip if need[4] else None, None, None, None, None, None)
@@ -369,7 +379,8 @@ class _GroupNormAct(torch.autograd.Function):
         call.keep = None        # what saves, offloads or recomputes saved tensors decides over their lives
         if not call.empty:
             call.backward_bytes = call.scratch_bytes(1)
-        ctx.call, ctx.rng = call, tuple(rng) if p and not device_rng else None      # (the caller may rewrite a list)
+        ctx.calls, ctx.args = [call], (groups, act, eps, p)
+        ctx.rng = tuple(rng) if p and not device_rng else None      # (the caller may rewrite a list)
         return y
 
     @staticmethod

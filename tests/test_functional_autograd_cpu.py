@@ -188,3 +188,30 @@ def test_statistics_that_come_back_with_other_strides(host, monkeypatch):
         [ctypes.c_float.from_address(stats + 4 * i).value for i in range(12)]))
     torch.autograd.grad(y, x, torch.ones_like(y))
     assert seen == [values.reshape(-1).tolist()]
+
+
+@pytest.mark.parametrize("spread", [1, 2], ids=["in place", "strided"])
+def test_a_backward_pass_that_finds_the_call_taken(host, spread):
+    """... by another thread describes its own from the saved tensors, to the same launch, and refuses the same."""
+    n, hw, c = 2, 6, 8
+    x, _, _ = _norm_inputs(n, hw, c, spread)
+    t = dict(x=x, skip=torch.randn(n, hw, c), weight=torch.ones(2 * c), bias=torch.zeros(2 * c), film=torch.zeros(n, 4 * c))
+    rng = torch.tensor([1, 2])
+    swap = [lambda s: s]
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: s, lambda s: swap[0](s)):
+        y = host.group_norm_act(groups=2, act="none", eps=1e-3, p=0.25, rng=rng, **t)
+    dy = torch.ones_like(y)
+    host.launches.clear()
+    for _ in range(2):
+        torch.autograd.grad(y, x, dy, retain_graph=True)
+        y.grad_fn.calls.clear()
+    (_, one), (_, two) = host.launches
+    assert bytes(one[0])[:-4] == bytes(two[0])[:-4] and one[1:3] == two[1:3] and one[-1] == two[-1]
+    host.launches.clear()
+    for bad in (lambda s: s.half() if s.is_floating_point() and s.dim() > 2 and s.shape[-1] > 2 else s,
+                lambda s: torch.cat([s, s], 1) if s.dim() > 2 and s.shape[-1] > 2 else s, lambda s: s[:1] if s.shape[0] == n else s):
+        y.grad_fn.calls.clear()
+        swap[0] = bad
+        with pytest.raises(ValueError):
+            torch.autograd.grad(y, x, dy, retain_graph=True)
+    assert not host.launches
