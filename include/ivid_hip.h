@@ -402,12 +402,13 @@ int ivid_sr_cond(const float* x, const float* y, float* out, int B, int Cx, int 
 int ivid_randn(unsigned long long seed, unsigned long long stream_id, float* out, long long n, void* stream);
 
 /* ---- dropout (nn.Dropout of a ResBlock, adm.py:181) from the same generator, the mask never stored ----
- * out[i] = kept(i) ? x[i] * 65536 / (65536 - T) : 0,  T = floor(p * 65536 + 1/2), kept(i) = draw(i) >= T: the expectation is x for
- * every p < 1 (p is used in steps of 2^-16); p = 1 drops all.  draw(i) = 16 bits, half i % 2 (low first) of word (i % 8) / 2 of the
- * Philox4x32-10 block with counter (i / 8, stream_id) and key seed ^ 0x44524F50 << 32: a pure function of (seed, stream_id, i), so the
- * backward pass is the same call on the gradient, and independent of ivid_randn's values for the same (seed, stream_id).
- * A dropped element is 0 whatever x holds.  x == out is allowed, another overlap is not.  rng: NULL, or device {seed, stream_id} read when the kernel runs
- * instead of the arguments (a captured graph then draws anew when the host rewrites them between replays). */
+ * out[i] = kept(i) ? x[i] * 65536 / (65536 - T) : 0,  T = floor(p * 65536 + 1/2), kept(i) = draw(i) >= T: p is used in steps of 2^-16,
+ * and the expectation is x for every T < 65536.  p >= 1 - 2^-17 is T = 65536 and drops all, p < 2^-17 is T = 0 and drops none.
+ * draw(i) = 16 bits, half i % 2 (low first) of word (i % 8) / 2 of the Philox4x32-10 block with counter (i / 8, stream_id) and key
+ * seed ^ 0x44524F50 << 32: a pure function of (seed, stream_id, i), so the backward pass is the same call on the gradient, and
+ * independent of ivid_randn's values for the same (seed, stream_id).  A dropped element is 0 whatever x holds.  x == out is allowed,
+ * another overlap is not.  rng: NULL, or device {seed, stream_id} read when the kernel runs instead of the arguments (a captured graph
+ * then draws anew when the host rewrites them between replays). */
 int ivid_dropout(int dtype, const void* x, void* out, long long n, double p, unsigned long long seed, unsigned long long stream_id,
                  const unsigned long long* rng, void* stream);
 

@@ -15,7 +15,9 @@
 //   * a wait ends after a bounded number of polls: the workgroup then computes the missing tile's sums itself, in the same order and
 //     so bit for bit the same, publishes them and goes on.  No workgroup depends on another one being resident.
 // A cluster of more than MAX_K tiles would not be resident at once: it takes two launches, sums and results (PH_SUMS, PH_RESULT), with
-// a small one between them that adds the words, and reads its inputs twice.
+// a small one between them that adds the words.  The second is the same code: it reads its inputs again and computes its tile's sums
+// again, which it then does not use.
+// The channels' sums of the tiles (backward) are added in 64 bits too, by launches behind the kernel.
 // Squares are centred on the tile's own means: a large mean costs no digits.
 //
 // Choices and what they measured (MI355X; 64 x 128 x 128 x 256 bf16; copying that tensor takes 202 us, 5.3 TB/s).  A variant's
@@ -49,7 +51,8 @@ constexpr int MAX_GS = 64;        // groups of a slab: at least four lanes each 
 constexpr int MAX_COL = 1024;     // channels of a tile
 constexpr int MAX_POLLS = 512;    // ~ 1 ms
 // Tiles of a cluster that runs as one launch: half of the 512 workgroups of a backward pass that the chip holds at once.  8 x 256 x 256 x
-// 128 bf16, one launch against two: backward (171 tiles) 134 us against 151, forward (64 tiles) 63 against 84.
+// 128 bf16, one launch against two (the second with its unused sums): backward (171 tiles) 134 us against 151, forward (64 tiles) 63
+// against 84.
 constexpr int MAX_K = 256;
 constexpr int MIN_TILES = 16;     // of a sample, once it is cut
 enum { PH_ALL = 0, PH_SUMS = 1, PH_RESULT = 2 };
@@ -966,7 +969,10 @@ int sweeps_for(int ve, int esz, bool backward, long long needed) {
   return list[i];
 }
 
-constexpr double TILES_COST = 2.2, SETUP_SWEEPS = 3.0;      // prices of the choice below, from measurements at 8 x 8 .. 128 x 128 pixels
+// Prices of the choice below, from measurements at 8 x 8 .. 128 x 128 pixels.  The choice by cost against a fixed one: 64 x 16 x 16 x 1792
+// fp16 forward 32 -> 27 us, backward 66 -> 56; 64 x 16 x 16 x 768 bf16 backward 37 -> 34; 64 x 8 x 8 x 1024 forward 12.2 -> 9.2;
+// 7 x 37 x 23 x 100 fp16 with dropout 20.8 -> 13.6.
+constexpr double TILES_COST = 2.2, SETUP_SWEEPS = 3.0;
 
 int cut_up(const ivid_gn_act_desc* d, bool backward, GnArgs* a, int* ve_out) {
   const int NT = backward ? NT_BWD : NT_FWD;

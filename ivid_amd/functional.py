@@ -20,7 +20,7 @@ not capture the backward pass of a graph that was built in eager code.
 Forward-mode derivatives do not exist here: tensors that carry a tangent (torch.autograd.forward_ad) are refused.
 
 Small training calls are bound by the host, and half of that is torch's change to its own thread for the backward pass: forward and
-gradients of a 7 x 37 x 23 x 100 tensor take 130 us, 67 under torch.autograd.set_multithreading_enabled(False).
+gradients of a 7 x 37 x 23 x 100 tensor take 130 us, 72 under torch.autograd.set_multithreading_enabled(False).
 """
 import ctypes as C
 import math
@@ -142,8 +142,9 @@ def dropout(x, p, rng=None):
     """y[i] = x[i] * 65536 / (65536 - T) where draw(i) >= T = floor(p * 65536 + 1/2), else 0; i = the row-major index.
 
     x any shape, float32 / bfloat16 / float16; other than contiguous tensors are copied first.  The draws are a function of (rng, i)
-    alone (include/ivid_hip.h ivid_dropout); a dropped element is 0 whatever x holds; p = 0 copies.  Under capture, and for the
-    gradient by hand, call it on the gradient with the same rng: the operator is its own backward pass."""
+    alone (include/ivid_hip.h ivid_dropout); a dropped element is 0 whatever x holds.  p is used in steps of 2^-16: below 2^-17 it
+    copies, from 1 - 2^-17 on it drops all; p = 0 needs no rng.  Under capture, and for the gradient by hand, call it on the gradient
+    with the same rng: the operator is its own backward pass."""
     _check_x(x, "x")
     p = _check_p(p)
     _refuse_tangents(x)

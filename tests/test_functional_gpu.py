@@ -751,3 +751,13 @@ def test_independent_of_the_batch_at_odd_sizes(shape, c0, c1, groups, dtype):
             for k in whole:
                 if k not in ("dweight", "dbias"):
                     assert torch.equal(whole[k][i:i + 1], got[k]), (k, i, copy)
+
+
+def test_dropout_probabilities_next_to_the_ends():
+    """p is used in steps of 2^-16, rounded to the nearest: less than half a step drops nothing, less than half a step below 1 all."""
+    x = randn(1, 1000)
+    assert torch.equal(F().dropout(x, 2.0 ** -17 * 0.99, RNG), x)
+    assert torch.equal(F().dropout(x, 1 - 2.0 ** -17, RNG), torch.zeros_like(x))
+    keep = R.drop_factor(1 << 20, 1 - 2.0 ** -16, RNG)
+    y = F().dropout(torch.ones(1 << 20, device="cuda"), 1 - 2.0 ** -16, RNG).double().cpu()
+    assert torch.equal(y, keep) and 0 < int((y != 0).sum()) < 100
